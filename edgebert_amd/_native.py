@@ -27,6 +27,9 @@ EBH_DTYPE_BF16 = 1
 EBH_DTYPE_F32_BF16X6 = 2
 NOALLOC_SCRATCH_BYTES = 128 << 20   # EBH_NOALLOC_SCRATCH_BYTES
 EPI_BIAS, EPI_BIAS_GELU, EPI_BIAS_RESID, EPI_NONE = 0, 1, 2, 3
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_NONE, ROPE_LINEAR, ROPE_NTK, ROPE_WAVELENGTH = 0, 1, 2, 3
+ACT_SILU, ACT_GELU_TANH, ACT_GELU_ERF = 0, 1, 2
 PROF = {"none": 0, "gemm_qkv": 1, "attention": 2, "gemm_out": 3, "gemm_ffn_up": 4,
         "gemm_ffn_down": 5, "layernorm": 6, "embed": 7, "pool": 8}
 
@@ -46,6 +49,12 @@ class EbhConfig(ctypes.Structure):
                 ("num_hidden_layers", ctypes.c_int32), ("intermediate_size", ctypes.c_int32),
                 ("vocab_size", ctypes.c_int32), ("max_position_embeddings", ctypes.c_int32),
                 ("type_vocab_size", ctypes.c_int32), ("layer_norm_eps", ctypes.c_float)]
+
+
+class EbhRope(ctypes.Structure):
+    _fields_ = [("rot_dim", ctypes.c_int32), ("layout", ctypes.c_int32), ("scaling", ctypes.c_int32),
+                ("original_len", ctypes.c_int32), ("base", ctypes.c_double), ("factor", ctypes.c_double),
+                ("turns_fast", ctypes.c_double), ("turns_slow", ctypes.c_double), ("magnitude", ctypes.c_double)]
 
 
 _vp = ctypes.c_void_p
@@ -104,6 +113,17 @@ _SIGS = {
     "ebh_op_f32_to_bf16": (_i32, [_vp, _vp, _i64, _vp]),
     "ebh_op_widen16": (_i32, [_vp, _vp, _i64, _i32, _vp]),
     "ebh_op_gelu": (_i32, [_vp, _vp, _i64, _vp]),
+    "ebh_op_rope": (_i32, [_vp, _i64, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, ctypes.POINTER(EbhRope), _i32, _vp]),
+    "ebh_op_layer_norm_fwd": (_i32, [_vp, _i64, _i32, _vp, _vp, _i32, _i32, _f32, _vp, _i64, _vp, _vp, _vp]),
+    "ebh_op_layer_norm_bwd_workspace": (_i64, [_i32, _i32]),
+    "ebh_op_layer_norm_bwd": (_i32, [_vp, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _i64, _vp,
+                                     _vp, _vp, _i64, _vp]),
+    "ebh_op_gated_ffn_workspace": (_i64, [_i32, _i32, _i32, _i32]),
+    "ebh_op_gated_ffn": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp,
+                                _i64, _vp]),
+    "ebh_op_gated_ffn_bwd_workspace": (_i64, [_i32, _i32, _i32, _i32]),
+    "ebh_op_gated_ffn_bwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i32, _i32,
+                                    _i32, _i32, _i32, _vp, _i64, _vp]),
 }
 
 _LIB = None

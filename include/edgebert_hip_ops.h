@@ -209,6 +209,114 @@ EBH_API int ebh_op_widen16(const uint16_t* x, void* y, int64_t n, int32_t mode, 
  * y[i] = gelu(x[i]) with the epilogue's exp2 + reciprocal evaluation. */
 EBH_API int ebh_op_gelu(const float* x, float* y, int64_t n, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * What a rotary, gated encoder layer adds: rotary positions, layer norm with
+ * gradients, and the gated feed-forward block with gradients.  dtype is
+ * EBH_DTYPE_F32 or EBH_DTYPE_BF16 (bf16 bits) and the type of every `void*`
+ * operand; statistics, biases, norm parameters and their gradients are fp32,
+ * and so are all sums.  Row strides (ld*) are in elements.  Outputs overlap no
+ * other operand unless said.  Calls allocate nothing and record kernels only
+ * (they may be captured); workspaces are the caller's, hold nothing between
+ * calls, and are used until the call's work is done: calls that may run at the
+ * same time, graphs that may be replayed at the same time among them, need one
+ * each.  `stream` and all operands belong to the current device.
+ * ------------------------------------------------------------------------- */
+
+/* Rotary positions.  Pair i of rot_dim / 2 of every head turns by angle
+ * pos * f_i: (a, b) -> magnitude (a cos - b sin, a sin + b cos).  Its columns
+ * are i and i + rot_dim / 2 of the head (EBH_ROPE_HALF) or 2 i and 2 i + 1
+ * (EBH_ROPE_INTERLEAVED); columns from rot_dim on pass unchanged.
+ * f_i = base^(-2 i / rot_dim), scaled for lengths beyond the trained one:
+ *   EBH_ROPE_LINEAR      f_i / factor;
+ *   EBH_ROPE_NTK         base * factor^(rot_dim / (rot_dim - 2)) in base's place;
+ *   EBH_ROPE_WAVELENGTH  f_i (g + (1 - g) / factor), g = (t - turns_slow) /
+ *       (turns_fast - turns_slow) clamped to 0 .. 1, where t = original_len *
+ *       f_i / (2 pi): pairs that turn often within the trained length keep
+ *       their frequency, slow ones are slowed by the factor.
+ * Fields that a scaling does not name are not read by it. */
+#define EBH_ROPE_HALF 0
+#define EBH_ROPE_INTERLEAVED 1
+#define EBH_ROPE_NONE 0
+#define EBH_ROPE_LINEAR 1
+#define EBH_ROPE_NTK 2
+#define EBH_ROPE_WAVELENGTH 3
+typedef struct ebh_rope {
+    int32_t rot_dim;      /* even, 2 .. head_dim */
+    int32_t layout;
+    int32_t scaling;
+    int32_t original_len; /* positions, > 0 (wavelength) */
+    double base;          /* > 0 */
+    double factor;        /* > 0 (linear, ntk, wavelength) */
+    double turns_fast, turns_slow; /* fast > slow (wavelength) */
+    double magnitude;     /* on the turned columns; 1: a rotation */
+} ebh_rope;
+
+/* y[t] = x[t] with its n_heads heads of head_dim columns turned to position
+ * pos[t] (any int32; ebh_op_pack's tok_pos); x's and y's rows are the first
+ * n_heads * head_dim columns of rows ldx and ldy apart, so one call turns q and
+ * k of a qkv row.  y may be x (ldy = ldx).  n_tokens (device, nullable): only the
+ * first *n_tokens of the T rows are turned, the others not read nor written.
+ * transpose != 0: the transposed map, angle -pos * f_i, which takes a
+ * gradient of y to one of x.  Angles are formed in 64 bits.  head_dim <= 1024,
+ * pointers aligned to their elements. */
+EBH_API int ebh_op_rope(const void* x, int64_t ldx, void* y, int64_t ldy, int32_t dtype, const int32_t* pos,
+                const int32_t* n_tokens, int32_t T, int32_t n_heads, int32_t head_dim, const ebh_rope* cfg,
+                int32_t transpose, void* stream);
+
+/* Layer norm over rows x [rows, H]: y = (x - mean) rstd gamma + beta, rstd = 1 /
+ * sqrt(var + eps), population variance; gamma and beta [H] may be NULL (1 and
+ * 0).  mean and rstd [rows] (nullable) are written for the backward pass.  y
+ * may be x (ldy = ldx).  H <= 16384, pointers aligned to their elements. */
+EBH_API int ebh_op_layer_norm_fwd(const void* x, int64_t ldx, int32_t dtype, const float* gamma, const float* beta,
+                          int32_t rows, int32_t H, float eps, void* y, int64_t ldy, float* mean, float* rstd,
+                          void* stream);
+
+/* Its backward pass: with xh = (x - mean) rstd and g = dy gamma,
+ * dx = rstd (g - mean_H(g) - xh mean_H(g xh)) + dres, dgamma = sum over rows of
+ * dy xh, dbeta = sum over rows of dy.  dres (nullable, row stride lddres) is a
+ * gradient that reaches x by another path.  dx may be dy, x or dres, with the
+ * same stride.  dgamma and dbeta [H] may be NULL; if either is not, `workspace`
+ * (16-byte aligned) holds ebh_op_layer_norm_bwd_workspace(rows, H) bytes, else it
+ * may be NULL.  No rows: dgamma and dbeta are zeros.  Results do not depend on
+ * timing. */
+EBH_API int64_t ebh_op_layer_norm_bwd_workspace(int32_t rows, int32_t H);
+EBH_API int ebh_op_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, int32_t dtype,
+                          const float* gamma, const float* mean, const float* rstd, const void* dres,
+                          int64_t lddres, int32_t rows, int32_t H, void* dx, int64_t lddx, float* dgamma,
+                          float* dbeta, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Gated feed-forward block: g | u = X.Wgu^T + bgu, h = act(g) u,
+ * Y = h.Wd^T + bd.  X [M, H] (ldx) and Y [M, H] (ldy); Wgu [2 I, H] holds the
+ * gate's I rows, then the other projection's; Wd [H, I]; biases (nullable) bgu
+ * [2 I], bd [H].  h [M, I] is written, and read by the second product; gu
+ * [M, 2 I] (nullable) keeps g | u for the backward pass.  Weights, h and gu are
+ * contiguous.  act: EBH_ACT_SILU g / (1 + e^-g), EBH_ACT_GELU_TANH (as
+ * EBH_EPI_BIAS_GELU) or EBH_ACT_GELU_ERF g/2 (1 + erf(g / sqrt 2)).  H, I and the
+ * strides are multiples of 8, H and I at most 65536, strides at most 2,796,202;
+ * operands 16-byte aligned.  `workspace` (16-byte aligned, NULL where 0) has
+ * ebh_op_gated_ffn_workspace(M, H, I, dtype) bytes. */
+#define EBH_ACT_SILU 0
+#define EBH_ACT_GELU_TANH 1
+#define EBH_ACT_GELU_ERF 2
+EBH_API int64_t ebh_op_gated_ffn_workspace(int32_t M, int32_t H, int32_t I, int32_t dtype);
+EBH_API int ebh_op_gated_ffn(const void* X, int64_t ldx, const void* Wgu, const float* bgu, const void* Wd,
+                     const float* bd, void* Y, int64_t ldy, void* h, void* gu, int32_t M, int32_t H, int32_t I,
+                     int32_t act, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Its backward pass, from dY [M, H] (lddy) and what the forward was given and
+ * kept: dh = dY.Wd, dg = dh u act'(g), du = dh act(g); dX = [dg du].Wgu (lddx),
+ * dWgu = [dg du]^T.X, dWd = dY^T.h, dbgu and dbd the column sums of [dg du] and
+ * dY.  Each of the five gradients may be NULL and is then not computed; weight
+ * gradients are contiguous.  [dg du] is rounded once to dtype for the products,
+ * and summed before that for dbgu.  No rows: weight and bias gradients are
+ * zeros.  Shapes, alignment and workspace (ebh_op_gated_ffn_bwd_workspace) as
+ * above.  Results do not depend on timing. */
+EBH_API int64_t ebh_op_gated_ffn_bwd_workspace(int32_t M, int32_t H, int32_t I, int32_t dtype);
+EBH_API int ebh_op_gated_ffn_bwd(const void* dY, int64_t lddy, const void* X, int64_t ldx, const void* h, const void* gu,
+                         const void* Wgu, const void* Wd, void* dX, int64_t lddx, void* dWgu, float* dbgu,
+                         void* dWd, float* dbd, int32_t M, int32_t H, int32_t I, int32_t act, int32_t dtype,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
