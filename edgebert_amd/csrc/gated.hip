@@ -1,189 +1,264 @@
 // gated.hip -- the gated feed-forward block and its gradients
-// (ebh_op_gated_ffn / _bwd).
+// (ebh_op_gated_ffn / _bwd), as products on the tiles of tile.hpp.
 #include <algorithm>
 
-#include "layer.hpp"
+#include "tile.hpp"
 
 namespace ebh {
 
-// Activation and its derivative.
-__device__ __forceinline__ float act_of(int act, float g) {
-    if (act == 0) return g / (1.0f + expf(-g));
-    if (act == 1) return gelu_tanh(g);
-    return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
-}
-__device__ __forceinline__ float act_slope(int act, float g) {
-    if (act == 0) {
-        const float s = 1.0f / (1.0f + expf(-g));
-        return s * (1.0f + g * (1.0f - s));
-    }
-    if (act == 1) {
-        const float t = tanhf(0.7978845608f * (g + 0.044715f * g * g * g));
-        return 0.5f * (1.0f + t) + 0.5f * g * (1.0f - t * t) * 0.7978845608f * (1.0f + 3.0f * 0.044715f * g * g);
-    }
-    return 0.5f * (1.0f + erff(g * 0.70710678118654752f)) + g * expf(-0.5f * g * g) * 0.3989422804014327f;
+// ---------------------------------------------------------------------------
+// The tiles, largest first.  A kernel's operand orders: both k contiguous
+// (forward), B strided (through the weights back), both strided (weight
+// gradients, whose k are the tokens).
+// ---------------------------------------------------------------------------
+template <class T, bool AKS, bool BKS, int TILE, int USE>
+__global__ __launch_bounds__(TILE == 0 ? 512 : 256, 2) void tile_kernel(TileArgs p) {
+    constexpr int BM = TILE == 0 ? 256 : (TILE == 1 ? 128 : 64), BN = TILE == 0 ? 256 : 128, NS = TILE == 2 ? 3 : 2;
+    __shared__ __attribute__((aligned(16))) char smem[tile_lds(BM, BN, NS)];
+    tile_body<T, AKS, BKS, BM, BN, 2, TILE == 0 ? 4 : 2, NS, USE>(p, smem);
 }
 
-// A product C(m, n) = sum over k of A(m, k) B(n, k) with operands in any
-// orders (element strides), and what becomes of it.
-enum Use : int { USE_STORE = 0, USE_GATE = 1, USE_SLOPES = 2 };
-struct SimpleArgs {
-    const void* A;
-    const void* B;
-    void* C;
-    int64_t am, ak, bn, bk, ldc;
-    int M, N, K;
-    const float* bias;
-    GatedArgs g;
-    float* colsum;      // USE_SLOPES: [row blocks][2 I] sums before rounding
-    void* dgu;
-};
-
-// 64 x 64 tiles, 16 x 16 threads of 4 x 4 outputs; USE_GATE: N = I, with a second
-// sum for the rows of B that are I further on.
-template <class T, int USE>
-__global__ __launch_bounds__(256) void simple_kernel(SimpleArgs p) {
-    __shared__ float sa[16][65], sb[16][65], sc[USE == USE_GATE ? 16 : 1][65];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int64_t m0 = (int64_t)blockIdx.y * 64, n0 = (int64_t)blockIdx.x * 64;
-    const T* A = static_cast<const T*>(p.A);
-    const T* B = static_cast<const T*>(p.B);
-    float acc[4][4] = {}, acc2[4][4] = {};
-    for (int k0 = 0; k0 < p.K; k0 += 16) {
-        for (int e = threadIdx.x; e < 1024; e += 256) {
-            const int r = e >> 4, k = e & 15;
-            const bool in = k0 + k < p.K;
-            sa[k][r] = in && m0 + r < p.M ? to_f32(A[(m0 + r) * p.am + (k0 + k) * p.ak]) : 0.0f;
-            sb[k][r] = in && n0 + r < p.N ? to_f32(B[(n0 + r) * p.bn + (k0 + k) * p.bk]) : 0.0f;
-            if (USE == USE_GATE) sc[k][r] = in && n0 + r < p.N ? to_f32(B[(n0 + r + p.N) * p.bn + (k0 + k) * p.bk]) : 0.0f;
-        }
-        __syncthreads();
-        for (int k = 0; k < 16; ++k)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) {
-                    acc[i][j] += sa[k][ty * 4 + i] * sb[k][tx * 4 + j];
-                    if (USE == USE_GATE) acc2[i][j] += sa[k][ty * 4 + i] * sc[k][tx * 4 + j];
-                }
-        __syncthreads();
-    }
-    float cg[4] = {}, cu[4] = {};
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-            if (m >= p.M || n >= p.N) continue;
-            const int64_t I = p.g.I;
-            if (USE == USE_STORE) {
-                store_as(static_cast<T*>(p.C) + m * p.ldc + n, acc[i][j] + (p.bias ? p.bias[n] : 0.0f));
-            } else if (USE == USE_GATE) {
-                const float g = acc[i][j] + (p.bias ? p.bias[n] : 0.0f), u = acc2[i][j] + (p.bias ? p.bias[I + n] : 0.0f);
-                store_as(static_cast<T*>(p.g.h) + m * I + n, act_of(p.g.act, g) * u);
-                if (p.g.gu) {
-                    store_as(static_cast<T*>(p.g.gu) + m * 2 * I + n, g);
-                    store_as(static_cast<T*>(p.g.gu) + m * 2 * I + I + n, u);
-                }
-            } else {
-                const T* gu = static_cast<const T*>(p.g.gu) + m * 2 * I + n;
-                const float g = to_f32(gu[0]), u = to_f32(gu[I]);
-                const float dg = acc[i][j] * u * act_slope(p.g.act, g), du = acc[i][j] * act_of(p.g.act, g);
-                T* out = static_cast<T*>(p.dgu) + m * 2 * I + n;
-                store_as(out, dg);
-                store_as(out + I, du);
-                cg[j] += dg;
-                cu[j] += du;
-            }
-        }
-    if (USE == USE_SLOPES && p.colsum) {
-        for (int j = 0; j < 4; ++j) {
-            sa[ty][tx * 4 + j] = cg[j];
-            sb[ty][tx * 4 + j] = cu[j];
-        }
-        __syncthreads();
-        if (threadIdx.x < 64 && n0 + threadIdx.x < p.N) {
-            float g = 0.0f, u = 0.0f;
-            for (int k = 0; k < 16; ++k) {
-                g += sa[k][threadIdx.x];
-                u += sb[k][threadIdx.x];
-            }
-            float* at = p.colsum + (int64_t)blockIdx.y * 2 * p.g.I + n0 + threadIdx.x;
-            at[0] = g;
-            at[p.g.I] = u;
-        }
-    }
-}
-
-// out[c] = sum over rows of x[r, c], in order of r.
+// out[part][c] = sum over the part's rows of x[., c]: 64 columns and 16 slices of
+// the rows a workgroup.
 template <class T>
-__global__ __launch_bounds__(256) void colsum_kernel(const T* x, int64_t ld, int rows, int cols, float* out) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= cols) return;
+__global__ __launch_bounds__(1024) void sum_rows_kernel(const T* x, int64_t ld, int64_t rows, int cols, float* out) {
+    __shared__ float part[16][64];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6;
+    const int64_t n = (int64_t)gridDim.y * 16, k = (int64_t)blockIdx.y * 16 + slice;
+    const int64_t r0 = rows * k / n, r1 = rows * (k + 1) / n;
     float s = 0.0f;
-    for (int64_t r = 0; r < rows; ++r) s += to_f32(x[r * ld + c]);
-    out[c] = s;
+    if (c < cols) {
+#pragma unroll 8
+        for (int64_t r = r0; r < r1; ++r) s += to_f32(x[r * ld + c]);
+    }
+    part[slice][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (slice == 0 && c < cols) {
+        s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s += part[i][threadIdx.x & 63];
+        out[(int64_t)blockIdx.y * cols + c] = s;
+    }
 }
 
-static int64_t up16(int64_t v) { return (v + 15) / 16 * 16; }
+// out = the sum of `parts` partial products, in order; n a multiple of 4.
+template <class T>
+__global__ __launch_bounds__(256) void sum_parts_kernel(const float* x, int parts, int64_t n, T* out) {
+    const int64_t i = 4 * (blockIdx.x * (int64_t)256 + threadIdx.x);
+    if (i >= n) return;
+    float4 s = *reinterpret_cast<const float4*>(x + i);
+    for (int k = 1; k < parts; ++k) {
+        const float4 v = *reinterpret_cast<const float4*>(x + k * n + i);
+        s.x += v.x;
+        s.y += v.y;
+        s.z += v.z;
+        s.w += v.w;
+    }
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(out + i) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
+    else *reinterpret_cast<float4*>(out + i) = s;
+}
+
+static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// Which tile: the largest that fills the chip, else ...
+static int pick_tile(int64_t M, int64_t N, bool f32, bool strided) {
+    const int cus = device_cu_count();
+    auto tiles = [&](int bm, int bn) { return (M + bm - 1) / bm * ((N + bn - 1) / bn); };
+    if (!f32 && tiles(256, 256) >= cus) return 0;
+    if (strided || tiles(128, 128) >= cus) return 1;
+    return 2;
+}
+
+struct SplitPlan {
+    int tile, splits, kt;
+};
+// Weight gradients: M x N products over `K` tokens.
+static SplitPlan plan_split(int64_t M, int64_t N, int K, bool bf16) {
+    const int cus = device_cu_count(), kt = (K + (bf16 ? 63 : 31)) / (bf16 ? 64 : 32);
+    const int tile = bf16 && M * N >= 256 * 256 * 4 && kt >= 64 ? 0 : 1;
+    const int bm = tile == 0 ? 256 : 128, slots = tile == 0 ? cus : 2 * cus;
+    const int64_t tiles = up(M, bm) / bm * (up(N, bm) / bm);
+    const int s = (int)std::max<int64_t>(1, std::min<int64_t>(slots / tiles, kt / 4));
+    SplitPlan p{tile, s, std::max(2, (int)up((kt + s - 1) / s, 2))};
+    p.splits = std::max(1, (kt + p.kt - 1) / p.kt);
+    return p;
+}
+
+template <class T, bool AKS, bool BKS, int USE>
+static void product(TileArgs a, int tile, hipStream_t s) {
+    constexpr int KT = 128 / sizeof(T);
+    if (a.splits == 0) {
+        a.splits = 1;
+        a.kt_split = std::max(2, (int)up((a.K + KT - 1) / KT, 2));
+    }
+    const int bm = tile == 0 ? 256 : (tile == 1 ? 128 : 64), bn = (tile == 0 ? 256 : 128) / (USE == USE_GATE ? 2 : 1);
+    const int64_t items = (int64_t)((a.M + bm - 1) / bm) * ((a.N + bn - 1) / bn) * a.splits;
+    const dim3 grid((unsigned)std::min<int64_t>(items, (int64_t)device_cu_count() * (tile == 0 ? 1 : 2)));
+    if constexpr (sizeof(T) == 2)
+        if (tile == 0) {
+            hipLaunchKernelGGL((tile_kernel<T, AKS, BKS, 0, USE>), grid, dim3(512), 0, s, a);
+            return;
+        }
+    if constexpr (!AKS)
+        if (tile == 2) {
+            hipLaunchKernelGGL((tile_kernel<T, AKS, BKS, 2, USE>), grid, dim3(256), 0, s, a);
+            return;
+        }
+    hipLaunchKernelGGL((tile_kernel<T, AKS, BKS, 1, USE>), grid, dim3(256), 0, s, a);
+}
+
+static int col_parts(int64_t rows) { return (int)std::max<int64_t>(1, std::min<int64_t>(64, rows / 256)); }
+template <class T>
+static void sum_rows(const T* x, int64_t ld, int64_t rows, int cols, float* parts, float* out, hipStream_t s) {
+    const int n = col_parts(rows);
+    const unsigned cb = (unsigned)((cols + 63) / 64);
+    hipLaunchKernelGGL((sum_rows_kernel<T>), dim3(cb, n), dim3(1024), 0, s, x, ld, rows, cols, n > 1 ? parts : out);
+    if (n > 1) hipLaunchKernelGGL((sum_rows_kernel<float>), dim3(cb), dim3(1024), 0, s, parts, (int64_t)cols, (int64_t)n, cols, out);
+}
+
+// The backward's workspace: [dg du], its column sums by row blocks, partial
+// weight gradients, and partial column sums.
+struct BwdSpace {
+    int64_t dgu, colsum, partial, cols, bytes;
+    SplitPlan wgu, wd;
+    int slopes_tile;
+};
+static BwdSpace bwd_space(int M, int H, int I, bool bf16) {
+    BwdSpace w;
+    const int64_t es = bf16 ? 2 : 4, I2 = 2 * (int64_t)I;
+    w.slopes_tile = pick_tile(M, I, !bf16, false);
+    const int bm = w.slopes_tile == 0 ? 256 : (w.slopes_tile == 1 ? 128 : 64);
+    w.wgu = plan_split(I2, H, M, bf16);
+    w.wd = plan_split(H, I, M, bf16);
+    int64_t at = up(M * I2 * es, 256);
+    w.dgu = 0;
+    w.colsum = at;
+    at += up((int64_t)((M + (int64_t)bm - 1) / bm) * 2 * I2 * 4, 256);
+    w.partial = at;
+    const int64_t pg = w.wgu.splits > 1 ? w.wgu.splits * I2 * H * 4 : 0, pd = w.wd.splits > 1 ? (int64_t)w.wd.splits * H * I * 4 : 0;
+    at += up(std::max(pg, pd), 256);
+    w.cols = at;
+    at += up(64 * std::max<int64_t>(I2, H) * 4, 256);
+    w.bytes = at;
+    return w;
+}
+
 int64_t gated_ws_bytes(int, int, int, bool) { return 0; }
-int64_t gated_bwd_ws_bytes(int M, int, int I, bool bf16) {
-    return up16((int64_t)M * 2 * I * (bf16 ? 2 : 4)) + ((int64_t)M + 63) / 64 * 2 * I * 4;
-}
-
-template <class T, int USE>
-static void product(SimpleArgs a, hipStream_t s) {
-    hipLaunchKernelGGL((simple_kernel<T, USE>), dim3((unsigned)((a.N + 63) / 64), (unsigned)((a.M + 63) / 64)), dim3(256), 0, s, a);
-}
+int64_t gated_bwd_ws_bytes(int M, int H, int I, bool bf16) { return bwd_space(M, H, I, bf16).bytes; }
 
 template <class T>
 static void gated(const GatedArgs& g, hipStream_t s) {
-    SimpleArgs a{};
-    a.g = g;
-    a.A = g.X; a.am = g.ldx; a.ak = 1;
-    a.B = g.Wgu; a.bn = g.H; a.bk = 1;
-    a.M = g.M; a.N = g.I; a.K = g.H;
+    constexpr bool F32 = sizeof(T) == 4;
+    TileArgs a{};
+    a.A = g.X;
+    a.lda = (int)g.ldx;
+    a.B = g.Wgu;
+    a.ldb = g.H;
+    a.M = g.M;
+    a.N = a.I = g.I;
+    a.K = g.H;
     a.bias = g.bgu;
-    product<T, USE_GATE>(a, s);
-    a.A = g.h; a.am = g.I;
-    a.B = g.Wd; a.bn = g.I;
-    a.C = g.Y; a.ldc = g.ldy;
-    a.N = g.H; a.K = g.I;
+    a.h = g.h;
+    a.gu = g.gu;
+    a.act = g.act;
+    product<T, false, false, USE_GATE>(a, pick_tile(g.M, 2 * (int64_t)g.I, F32, false), s);
+    a.A = g.h;
+    a.lda = g.I;
+    a.B = g.Wd;
+    a.ldb = g.I;
+    a.C = g.Y;
+    a.ldc = (int)g.ldy;
+    a.N = g.H;
+    a.K = g.I;
     a.bias = g.bd;
-    product<T, USE_STORE>(a, s);
+    product<T, false, false, USE_STORE>(a, pick_tile(g.M, g.H, F32, false), s);
+}
+
+template <class T>
+static void weight_gradient(TileArgs a, const SplitPlan& w, float* partial, void* out, hipStream_t s) {
+    a.splits = w.splits;
+    a.kt_split = w.kt;
+    a.ldc = a.N;
+    a.bias = nullptr;
+    if (w.splits == 1) {
+        a.C = out;
+        product<T, true, true, USE_STORE>(a, w.tile, s);
+        return;
+    }
+    a.C = partial;
+    product<T, true, true, USE_PARTIAL>(a, w.tile, s);
+    const int64_t n = (int64_t)a.M * a.N;
+    hipLaunchKernelGGL((sum_parts_kernel<T>), dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, s, partial, w.splits, n, static_cast<T*>(out));
 }
 
 template <class T>
 static void gated_bwd(const GatedArgs& g, hipStream_t s) {
-    SimpleArgs a{};
-    a.g = g;
-    a.dgu = g.ws;
+    constexpr bool F32 = sizeof(T) == 4;
+    const BwdSpace w = bwd_space(g.M, g.H, g.I, !F32);
+    char* const ws = static_cast<char*>(g.ws);
     const int64_t I2 = 2 * (int64_t)g.I;
-    a.colsum = reinterpret_cast<float*>(static_cast<char*>(g.ws) + up16(g.M * I2 * sizeof(T)));
-    a.A = g.dY; a.am = g.lddy; a.ak = 1;
-    a.B = g.Wd; a.bn = 1; a.bk = g.I;
-    a.M = g.M; a.N = g.I; a.K = g.H;
-    if (g.M > 0) product<T, USE_SLOPES>(a, s);
-    if (g.dbgu)
-        hipLaunchKernelGGL((colsum_kernel<float>), dim3((unsigned)((I2 + 255) / 256)), dim3(256), 0, s, a.colsum, I2, (g.M + 63) / 64, (int)I2, g.dbgu);
-    if (g.dbd)
-        hipLaunchKernelGGL((colsum_kernel<T>), dim3((unsigned)((g.H + 255) / 256)), dim3(256), 0, s, static_cast<const T*>(g.dY), g.lddy, g.M, g.H, g.dbd);
-    if (g.dX && g.M > 0) {
-        a.A = g.ws; a.am = I2; a.ak = 1;
-        a.B = g.Wgu; a.bn = 1; a.bk = g.H;
-        a.C = g.dX; a.ldc = g.lddx;
-        a.N = g.H; a.K = (int)I2;
-        product<T, USE_STORE>(a, s);
+    if (g.M == 0) {   // sums over no rows
+        const int64_t es = sizeof(T) / 2;   // in 16-bit halves of words
+        if (g.dWgu) launch_zero_words(g.dWgu, I2 * g.H * es / 2, s);
+        if (g.dWd) launch_zero_words(g.dWd, (int64_t)g.H * g.I * es / 2, s);
+        if (g.dbgu) launch_zero_words(g.dbgu, I2, s);
+        if (g.dbd) launch_zero_words(g.dbd, g.H, s);
+        return;
     }
+    float* const colsum = reinterpret_cast<float*>(ws + w.colsum);
+    float* const partial = reinterpret_cast<float*>(ws + w.partial);
+    float* const cols = reinterpret_cast<float*>(ws + w.cols);
+    TileArgs a{};
+    a.act = g.act;
+    a.I = g.I;
+    if (g.dX || g.dWgu || g.dbgu) {
+        a.A = g.dY;
+        a.lda = (int)g.lddy;
+        a.B = g.Wd;
+        a.ldb = g.I;
+        a.M = g.M;
+        a.N = g.I;
+        a.K = g.H;
+        a.gu = g.gu;
+        a.dgu = ws;
+        a.colsum = g.dbgu ? colsum : nullptr;
+        product<T, false, true, USE_SLOPES>(a, w.slopes_tile, s);
+        if (g.dbgu) {
+            const int bm = w.slopes_tile == 0 ? 256 : (w.slopes_tile == 1 ? 128 : 64);
+            sum_rows<float>(colsum, I2, (g.M + (int64_t)bm - 1) / bm * 2, (int)I2, cols, g.dbgu, s);
+        }
+    }
+    if (g.dbd) sum_rows<T>(static_cast<const T*>(g.dY), g.lddy, g.M, g.H, cols, g.dbd, s);
+    if (g.dX) {
+        a.A = ws;
+        a.lda = (int)I2;
+        a.B = g.Wgu;
+        a.ldb = g.H;
+        a.C = g.dX;
+        a.ldc = (int)g.lddx;
+        a.M = g.M;
+        a.N = g.H;
+        a.K = (int)I2;
+        product<T, false, true, USE_STORE>(a, pick_tile(g.M, g.H, F32, false), s);
+    }
+    a.K = g.M;
     if (g.dWgu) {
-        a.A = g.ws; a.am = 1; a.ak = I2;
-        a.B = g.X; a.bn = 1; a.bk = g.ldx;
-        a.C = g.dWgu; a.ldc = g.H;
-        a.M = (int)I2; a.N = g.H; a.K = g.M;
-        product<T, USE_STORE>(a, s);
+        a.A = ws;
+        a.lda = (int)I2;
+        a.B = g.X;
+        a.ldb = (int)g.ldx;
+        a.M = (int)I2;
+        a.N = g.H;
+        weight_gradient<T>(a, w.wgu, partial, g.dWgu, s);
     }
     if (g.dWd) {
-        a.A = g.dY; a.am = 1; a.ak = g.lddy;
-        a.B = g.h; a.bn = 1; a.bk = g.I;
-        a.C = g.dWd; a.ldc = g.I;
-        a.M = g.H; a.N = g.I; a.K = g.M;
-        product<T, USE_STORE>(a, s);
+        a.A = g.dY;
+        a.lda = (int)g.lddy;
+        a.B = g.h;
+        a.ldb = g.I;
+        a.M = g.H;
+        a.N = g.I;
+        weight_gradient<T>(a, w.wd, partial, g.dWd, s);
     }
 }
 
