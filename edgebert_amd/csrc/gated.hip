@@ -11,11 +11,23 @@ namespace ebh {
 // (forward), B strided (through the weights back), both strided (weight
 // gradients, whose k are the tokens).
 // ---------------------------------------------------------------------------
+struct TileShape {
+    int bm, bn, waves_m, waves_n, ns;
+};
+constexpr int TILES = 4, TILE_KB = 128;
+constexpr TileShape kTiles[TILES] = {
+    {256, 256, 2, 4, 2},   // 8 waves, one workgroup a CU
+    {256, 192, 4, 2, 2},
+    {128, 128, 2, 2, 2},   // 4 waves, two a CU
+    {64, 128, 2, 2, 3},
+};
+constexpr int tile_threads(int t) { return 64 * kTiles[t].waves_m * kTiles[t].waves_n; }
+
 template <class T, bool AKS, bool BKS, int TILE, int USE>
-__global__ __launch_bounds__(TILE == 0 ? 512 : 256, 2) void tile_kernel(TileArgs p) {
-    constexpr int BM = TILE == 0 ? 256 : (TILE == 1 ? 128 : 64), BN = TILE == 0 ? 256 : 128, NS = TILE == 2 ? 3 : 2;
-    __shared__ __attribute__((aligned(16))) char smem[tile_lds(BM, BN, NS)];
-    tile_body<T, AKS, BKS, BM, BN, 2, TILE == 0 ? 4 : 2, NS, USE>(p, smem);
+__global__ __launch_bounds__(tile_threads(TILE), 2) void tile_kernel(TileArgs p) {
+    constexpr TileShape S = kTiles[TILE];
+    __shared__ __attribute__((aligned(16))) char smem[tile_lds<BKS, S.bm, S.bn, TILE_KB, S.ns>()];
+    tile_body<T, AKS, BKS, S.bm, S.bn, S.waves_m, S.waves_n, TILE_KB, S.ns, USE>(p, smem);
 }
 
 // out[part][c] = sum over the part's rows of x[., c]: 64 columns and 16 slices of
@@ -41,70 +53,136 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(const T* x, int64_t ld, 
     }
 }
 
-// out = the sum of `parts` partial products, in order; n a multiple of 4.
+// out = the sum of `parts` partial products of n4 x 4 elements, in order, + bias;
+// rows of cols4 x 4 elements, ld apart.
 template <class T>
-__global__ __launch_bounds__(256) void sum_parts_kernel(const float* x, int parts, int64_t n, T* out) {
-    const int64_t i = 4 * (blockIdx.x * (int64_t)256 + threadIdx.x);
-    if (i >= n) return;
-    float4 s = *reinterpret_cast<const float4*>(x + i);
+__global__ __launch_bounds__(256) void sum_parts_kernel(const float4* x, int parts, uint32_t n4, uint32_t cols4, const float* bias, T* out, int ld) {
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= n4) return;
+    float4 s = x[i];
+#pragma unroll 4
     for (int k = 1; k < parts; ++k) {
-        const float4 v = *reinterpret_cast<const float4*>(x + k * n + i);
+        const float4 v = x[(int64_t)k * n4 + i];
         s.x += v.x;
         s.y += v.y;
         s.z += v.z;
         s.w += v.w;
     }
-    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(out + i) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
-    else *reinterpret_cast<float4*>(out + i) = s;
+    const uint32_t row = i / cols4, c = 4 * (i - row * cols4);
+    if (bias) {
+        s.x += bias[c];
+        s.y += bias[c + 1];
+        s.z += bias[c + 2];
+        s.w += bias[c + 3];
+    }
+    T* const o = out + (int64_t)row * ld + c;
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
+    else *reinterpret_cast<float4*>(o) = s;
 }
 
 static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// Which tile: the largest that fills the chip, else ...
-static int pick_tile(int64_t M, int64_t N, bool f32, bool strided) {
-    const int cus = device_cu_count();
-    auto tiles = [&](int bm, int bn) { return (M + bm - 1) / bm * ((N + bn - 1) / bn); };
-    if (!f32 && tiles(256, 256) >= cus) return 0;
-    if (strided || tiles(128, 128) >= cus) return 1;
-    return 2;
+// ---------------------------------------------------------------------------
+// The choice of a tile and of splits over k, by estimated time: with n items on
+// the busiest CU, rounds of one workgroup a CU (tiles 0 and 1) or of two, us:
+//   launch + full rounds * (k/64 * full + epi) + a last one of one workgroup
+//   (k/64 * one + epi / 2).
+// Constants fitted to a sweep on MI355X of the five products at 70 .. 32,768
+// tokens of H 384 .. 1,024, I 1,000 .. 4,096 and 1 .. 24 splits (rms error 4-14%;
+// the choice takes 1.01-1.02 times the best's time on average, at worst 1.23).
+// What they say: the largest tile runs its k fastest but needs whole rounds of
+// 256; few tiles are split over k, as long as writing and reading the partial
+// sums (6 TB/s, and a launch) costs less than the idle CUs.
+// ---------------------------------------------------------------------------
+struct TileTime {
+    float launch, full, epi, one;
+};
+static const TileTime kTimes[2][4][TILES] = {   // bf16, fp32; by Use
+    {{{0.0f, 1.333f, 8.7f, 0}, {0.0f, 1.113f, 7.0f, 0}, {0.0f, 0.826f, 6.6f, 0.639f}, {4.2f, 0.629f, 1.3f, 0.434f}},
+     {{1.8f, 1.373f, 11.0f, 0}, {3.3f, 1.165f, 7.7f, 0}, {2.6f, 0.882f, 5.0f, 0.647f}, {3.7f, 0.619f, 2.2f, 0.412f}},
+     {{2.9f, 1.453f, 5.3f, 0}, {}, {3.5f, 1.086f, 0.6f, 0.646f}, {2.8f, 0.907f, 0.0f, 0.614f}},
+     {{0.0f, 1.337f, 20.5f, 0}, {}, {0.1f, 0.737f, 14.4f, 0.512f}, {2.2f, 0.729f, 4.8f, 0.504f}}},
+    {{{}, {}, {5.5f, 7.39f, 4.0f, 3.963f}, {0.0f, 4.119f, 5.4f, 2.489f}},
+     {{}, {}, {3.9f, 7.389f, 3.8f, 3.994f}, {3.8f, 4.013f, 1.8f, 2.374f}},
+     {{}, {}, {0.0f, 6.766f, 10.4f, 3.953f}, {3.2f, 3.886f, 3.1f, 2.360f}},
+     {{}, {}, {0.2f, 6.804f, 23.2f, 3.665f}, {0.0f, 3.202f, 13.9f, 2.352f}}},
+};
+
+// Whether a product can have a tile: fp32 tiles are the small ones; a strided A has
+// at least 128 columns; the gate's waves have pairs of blocks of each projection.
+constexpr bool has_tile(int t, bool bf16, bool a_strided, int use) {
+    return (bf16 || t >= 2) && !(a_strided && t == 3) && !(t == 1 && (use == USE_GATE || use == USE_SLOPES));
 }
 
-struct SplitPlan {
-    int tile, splits, kt;
+struct Plan {
+    int tile, splits, kt_split;
+    int64_t partial;   // bytes of partial sums
 };
-// Weight gradients: M x N products over `K` tokens.
-static SplitPlan plan_split(int64_t M, int64_t N, int K, bool bf16) {
-    const int cus = device_cu_count(), kt = (K + (bf16 ? 63 : 31)) / (bf16 ? 64 : 32);
-    const int tile = bf16 && M * N >= 256 * 256 * 4 && kt >= 64 ? 0 : 1;
-    const int bm = tile == 0 ? 256 : 128, slots = tile == 0 ? cus : 2 * cus;
-    const int64_t tiles = up(M, bm) / bm * (up(N, bm) / bm);
-    const int s = (int)std::max<int64_t>(1, std::min<int64_t>(slots / tiles, kt / 4));
-    SplitPlan p{tile, s, std::max(2, (int)up((kt + s - 1) / s, 2))};
-    p.splits = std::max(1, (kt + p.kt - 1) / p.kt);
-    return p;
+
+// An M x N product over K; most: bytes of partial sums there may be.
+static Plan plan_product(int64_t M, int64_t N, int64_t K, bool bf16, bool a_strided, int use, int64_t most) {
+    const int cus = device_cu_count(), KT = TILE_KB / (bf16 ? 2 : 4);
+    const int64_t nk = std::max<int64_t>(2, up((K + KT - 1) / KT, 2));
+    Plan best{0, 1, (int)nk, 0};
+    double best_us = 1e30;
+    for (int S : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24}) {
+        const int64_t per_split = up((nk + S - 1) / S, 2), bytes = S > 1 ? (int64_t)S * M * N * 4 : 0;
+        if (S > 1 && (most <= 0 || bytes > most || (nk + per_split - 1) / per_split != S)) continue;
+        for (int t = 0; t < TILES; ++t) {
+            if (!has_tile(t, bf16, a_strided, use)) continue;
+            const TileTime& c = kTimes[bf16 ? 0 : 1][S > 1 ? USE_PARTIAL : use][t];
+            const int bn = kTiles[t].bn / (use == USE_GATE ? 2 : 1);
+            const int64_t per = ((M + kTiles[t].bm - 1) / kTiles[t].bm * ((N + bn - 1) / bn) * S + cus - 1) / cus;
+            const int64_t full = t < 2 ? per : per / 2, rem = t < 2 ? 0 : per & 1;
+            const double k = (double)per_split * KT / 64.0;
+            double us = c.launch + full * (k * c.full + c.epi) + rem * (k * c.one + 0.5 * c.epi);
+            if (S > 1) us += 3.0 + bytes / 6.0e6;
+            if (us < best_us) {
+                best_us = us;
+                best = Plan{t, S, (int)per_split, bytes};
+            }
+        }
+    }
+    return best;
+}
+
+// Launches tile t of those that a product can have.
+template <class T, bool AKS, bool BKS, int USE, int TILE = 0>
+static void launch_tile(const TileArgs& a, int t, dim3 grid, hipStream_t s) {
+    if constexpr (TILE < TILES) {
+        if constexpr (has_tile(TILE, sizeof(T) == 2, AKS, USE))
+            if (t == TILE) {
+                hipLaunchKernelGGL((tile_kernel<T, AKS, BKS, TILE, USE>), grid, dim3(tile_threads(TILE)), 0, s, a);
+                return;
+            }
+        launch_tile<T, AKS, BKS, USE, TILE + 1>(a, t, grid, s);
+    }
 }
 
 template <class T, bool AKS, bool BKS, int USE>
-static void product(TileArgs a, int tile, hipStream_t s) {
-    constexpr int KT = 128 / sizeof(T);
-    if (a.splits == 0) {
-        a.splits = 1;
-        a.kt_split = std::max(2, (int)up((a.K + KT - 1) / KT, 2));
+static void product(TileArgs a, const Plan& w, hipStream_t s) {
+    a.splits = w.splits;
+    a.kt_split = w.kt_split;
+    const int bm = kTiles[w.tile].bm, bn = kTiles[w.tile].bn / (USE == USE_GATE ? 2 : 1);
+    const int64_t items = ((int64_t)a.M + bm - 1) / bm * ((a.N + bn - 1) / bn) * a.splits;
+    launch_tile<T, AKS, BKS, USE>(a, w.tile, dim3((unsigned)std::min<int64_t>(items, (int64_t)device_cu_count() * (w.tile < 2 ? 1 : 2))), s);
+}
+
+// C = A.B (+ bias), by way of partial sums where the plan splits k.
+template <class T, bool AKS, bool BKS>
+static void stored_product(TileArgs a, const Plan& w, float* partial, hipStream_t s) {
+    if (w.splits == 1) {
+        product<T, AKS, BKS, USE_STORE>(a, w, s);
+        return;
     }
-    const int bm = tile == 0 ? 256 : (tile == 1 ? 128 : 64), bn = (tile == 0 ? 256 : 128) / (USE == USE_GATE ? 2 : 1);
-    const int64_t items = (int64_t)((a.M + bm - 1) / bm) * ((a.N + bn - 1) / bn) * a.splits;
-    const dim3 grid((unsigned)std::min<int64_t>(items, (int64_t)device_cu_count() * (tile == 0 ? 1 : 2)));
-    if constexpr (sizeof(T) == 2)
-        if (tile == 0) {
-            hipLaunchKernelGGL((tile_kernel<T, AKS, BKS, 0, USE>), grid, dim3(512), 0, s, a);
-            return;
-        }
-    if constexpr (!AKS)
-        if (tile == 2) {
-            hipLaunchKernelGGL((tile_kernel<T, AKS, BKS, 2, USE>), grid, dim3(256), 0, s, a);
-            return;
-        }
-    hipLaunchKernelGGL((tile_kernel<T, AKS, BKS, 1, USE>), grid, dim3(256), 0, s, a);
+    T* const out = static_cast<T*>(a.C);
+    const int ld = a.ldc;
+    a.C = partial;
+    a.ldc = a.N;
+    product<T, AKS, BKS, USE_PARTIAL>(a, w, s);
+    const uint32_t n4 = (uint32_t)((int64_t)a.M * a.N / 4);
+    hipLaunchKernelGGL((sum_parts_kernel<T>), dim3((n4 + 255) / 256), dim3(256), 0, s, reinterpret_cast<const float4*>(partial), w.splits, n4,
+                       (uint32_t)(a.N / 4), a.bias, out, ld);
 }
 
 static int col_parts(int64_t rows) { return (int)std::max<int64_t>(1, std::min<int64_t>(64, rows / 256)); }
@@ -116,39 +194,187 @@ static void sum_rows(const T* x, int64_t ld, int64_t rows, int cols, float* part
     if (n > 1) hipLaunchKernelGGL((sum_rows_kernel<float>), dim3(cb), dim3(1024), 0, s, parts, (int64_t)cols, (int64_t)n, cols, out);
 }
 
-// The backward's workspace: [dg du], its column sums by row blocks, partial
-// weight gradients, and partial column sums.
-struct BwdSpace {
-    int64_t dgu, colsum, partial, cols, bytes;
-    SplitPlan wgu, wd;
-    int slopes_tile;
+// ---------------------------------------------------------------------------
+// At most FEW_ROWS tokens, where the weights' bytes are the work: a workgroup has
+// 16 columns and all of k, every 128 bytes of a weight row go to one wave as 32
+// contiguous bytes a lane, straight into MFMA operands, and each wave sums its
+// share of k; the waves' sums meet in LDS.  X comes from the caches.
+// ---------------------------------------------------------------------------
+constexpr int FEW_ROWS = 64;
+struct FewArgs {
+    const void* X;      // [M, K], fp32 where it is split
+    const void* W;      // [N, K] rows; the gate's and then the other projection's where GATE
+    const float* bias;
+    void* out;          // h or Y
+    void* gu;           // GATE: [M, 2 N], or null
+    float* hf;          // GATE, bf16: h before its rounding
+    int M, N, K, ldx, ldo, act;
 };
-static BwdSpace bwd_space(int M, int H, int I, bool bf16) {
-    BwdSpace w;
-    const int64_t es = bf16 ? 2 : 4, I2 = 2 * (int64_t)I;
-    w.slopes_tile = pick_tile(M, I, !bf16, false);
-    const int bm = w.slopes_tile == 0 ? 256 : (w.slopes_tile == 1 ? 128 : 64);
-    w.wgu = plan_split(I2, H, M, bf16);
-    w.wd = plan_split(H, I, M, bf16);
-    int64_t at = up(M * I2 * es, 256);
-    w.dgu = 0;
-    w.colsum = at;
-    at += up((int64_t)((M + (int64_t)bm - 1) / bm) * 2 * I2 * 4, 256);
-    w.partial = at;
-    const int64_t pg = w.wgu.splits > 1 ? w.wgu.splits * I2 * H * 4 : 0, pd = w.wd.splits > 1 ? (int64_t)w.wd.splits * H * I * 4 : 0;
-    at += up(std::max(pg, pd), 256);
-    w.cols = at;
-    at += up(64 * std::max<int64_t>(I2, H) * 4, 256);
-    w.bytes = at;
-    return w;
+
+// SPLIT: X is fp32, and each value is two bf16 (16 of its bits: the products'
+// operand errors are 2^-17 instead of 2^-9; the MFMAs are idle anyway).
+template <class T, int MB, bool GATE, bool SPLIT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void few_kernel(FewArgs p) {
+    constexpr int ES = sizeof(T), KT = 128 / ES, CE = 16 / ES, G = GATE ? 2 : 1, PASS = MB > 2 ? 2 : 4, XP = SPLIT ? 2 : 1;
+    __shared__ __attribute__((aligned(16))) float red[WAVES * MB * G * 256];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, q = lane >> 4;
+    const int n0 = blockIdx.x * 16;
+    typedef std::conditional_t<SPLIT, float, T> TX;
+    const T* const w0 = static_cast<const T*>(p.W) + (int64_t)min(n0 + r, p.N - 1) * p.K;
+    const TX* x[MB];
+#pragma unroll
+    for (int b = 0; b < MB; ++b) x[b] = static_cast<const TX*>(p.X) + (int64_t)min(16 * b + r, p.M - 1) * p.ldx;
+    g16_v4f acc[G][MB];
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int b = 0; b < MB; ++b) acc[g][b] = g16_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    const int chunks = (p.K + KT - 1) / KT;
+    for (int c0 = wave; c0 < chunks; c0 += WAVES * PASS) {
+        g16_v4f wv[PASS][G][2], xv[PASS][MB][2][XP];
+#pragma unroll
+        for (int u = 0; u < PASS; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int k = (c0 + u * WAVES) * KT + q * (KT / 4) + h * CE;   // K is whole pieces of CE
+                const bool in = k < p.K;
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+                    wv[u][g][h] = in ? *reinterpret_cast<const g16_v4f*>(w0 + (int64_t)g * p.N * p.K + k) : g16_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int b = 0; b < MB; ++b)
+#pragma unroll
+                    for (int e = 0; e < XP; ++e)
+                        xv[u][b][h][e] = in ? *reinterpret_cast<const g16_v4f*>(x[b] + k + 4 * e) : g16_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+#pragma unroll
+        for (int u = 0; u < PASS; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int b = 0; b < MB; ++b) {
+                    if constexpr (SPLIT) {
+                        const g16_v4f a = xv[u][b][h][0], c = xv[u][b][h][1];
+                        u4v_t hi = {pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(c[0], c[1]), pack_bf16x2(c[2], c[3])}, lo;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float v0 = e < 2 ? a[2 * e] : c[2 * e - 4], v1 = e < 2 ? a[2 * e + 1] : c[2 * e - 3];
+                            lo[e] = pack_bf16x2(v0 - __uint_as_float(hi[e] << 16), v1 - __uint_as_float(hi[e] & 0xffff0000u));
+                        }
+                        acc[0][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(g16_v8bf, wv[u][0][h]), __builtin_bit_cast(g16_v8bf, lo),
+                                                                            acc[0][b], 0, 0, 0);
+                        acc[0][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(g16_v8bf, wv[u][0][h]), __builtin_bit_cast(g16_v8bf, hi),
+                                                                            acc[0][b], 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int g = 0; g < G; ++g) {
+                            if constexpr (ES == 2)
+                                acc[g][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(g16_v8bf, wv[u][g][h]),
+                                                                                    __builtin_bit_cast(g16_v8bf, xv[u][b][h][0]), acc[g][b], 0, 0, 0);
+                            else
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    acc[g][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv[u][g][h][e], xv[u][b][h][0][e], acc[g][b], 0, 0, 0);
+                        }
+                    }
+                }
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int b = 0; b < MB; ++b) *reinterpret_cast<g16_v4f*>(red + ((wave * MB + b) * G + g) * 256 + r * 16 + 4 * q) = acc[g][b];
+    __syncthreads();
+    // four columns of a row a thread
+    if (tid >= MB * 64) return;
+    const int b = tid >> 6, row = 16 * b + r, n = n0 + 4 * q;
+    if (row >= p.M || n >= p.N) return;
+    g16_v4f v[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        v[g] = *reinterpret_cast<const g16_v4f*>(red + (b * G + g) * 256 + r * 16 + 4 * q);
+        for (int w = 1; w < WAVES; ++w) v[g] += *reinterpret_cast<const g16_v4f*>(red + ((w * MB + b) * G + g) * 256 + r * 16 + 4 * q);
+        if (p.bias) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[g][e] += p.bias[g * p.N + n + e];
+        }
+    }
+    auto put = [&](void* base, int64_t at, const g16_v4f& o) __attribute__((always_inline)) {
+        if constexpr (ES == 2) *reinterpret_cast<uint2*>(static_cast<T*>(base) + at) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+        else *reinterpret_cast<g16_v4f*>(static_cast<T*>(base) + at) = o;
+    };
+    if constexpr (GATE) {
+        float gv[4] = {v[0][0], v[0][1], v[0][2], v[0][3]}, uv[4] = {v[1][0], v[1][1], v[1][2], v[1][3]}, hv[4];
+        act_times<4>(p.act, gv, uv, hv);
+        const g16_v4f h = {hv[0], hv[1], hv[2], hv[3]};
+        put(p.out, (int64_t)row * p.N + n, h);
+        if (p.hf) *reinterpret_cast<g16_v4f*>(p.hf + (int64_t)row * p.N + n) = h;
+        if (p.gu) {
+            put(p.gu, (int64_t)row * 2 * p.N + n, v[0]);
+            put(p.gu, (int64_t)row * 2 * p.N + p.N + n, v[1]);
+        }
+    } else {
+        put(p.out, (int64_t)row * p.ldo + n, v[0]);
+    }
 }
 
-int64_t gated_ws_bytes(int, int, int, bool) { return 0; }
-int64_t gated_bwd_ws_bytes(int M, int H, int I, bool bf16) { return bwd_space(M, H, I, bf16).bytes; }
+template <class T, bool GATE, bool SPLIT>
+static void launch_few(const FewArgs& a, hipStream_t s) {
+    // 4 waves and 32 columns' rows, or 8 and 16: as many bytes on their way
+    constexpr int WAVES = GATE ? 4 : 8;
+    const dim3 grid((unsigned)((a.N + 15) / 16)), block(64 * WAVES);
+    switch ((a.M + 15) / 16) {
+        case 1: hipLaunchKernelGGL((few_kernel<T, 1, GATE, SPLIT, WAVES>), grid, block, 0, s, a); break;
+        case 2: hipLaunchKernelGGL((few_kernel<T, 2, GATE, SPLIT, WAVES>), grid, block, 0, s, a); break;
+        case 3: hipLaunchKernelGGL((few_kernel<T, 3, GATE, SPLIT, WAVES>), grid, block, 0, s, a); break;
+        default: hipLaunchKernelGGL((few_kernel<T, 4, GATE, SPLIT, WAVES>), grid, block, 0, s, a); break;
+    }
+}
+
+template <class T>
+static void few(const GatedArgs& g, hipStream_t s) {
+    constexpr bool BF16 = sizeof(T) == 2;
+    FewArgs a{};
+    a.X = g.X;
+    a.ldx = (int)g.ldx;
+    a.W = g.Wgu;
+    a.bias = g.bgu;
+    a.out = g.h;
+    a.gu = g.gu;
+    a.hf = BF16 ? static_cast<float*>(g.ws) : nullptr;
+    a.M = g.M;
+    a.N = g.I;
+    a.K = g.H;
+    a.act = g.act;
+    launch_few<T, true, false>(a, s);
+    a.X = BF16 ? g.ws : g.h;
+    a.ldx = g.I;
+    a.W = g.Wd;
+    a.bias = g.bd;
+    a.out = g.Y;
+    a.ldo = (int)g.ldy;
+    a.N = g.H;
+    a.K = g.I;
+    launch_few<T, false, BF16>(a, s);
+}
+
+// Most bytes of partial sums: of outputs of a row a token, and of weights' gradients.
+constexpr int64_t PARTIAL_ROWS = 64 << 20, PARTIAL_WEIGHTS = 512 << 20;
+
+// At most FEW_ROWS tokens: few_kernel reads the weights once and needs no tiles.
+// bf16: its h between the two products is kept in fp32 too, in the workspace.
+static Plan down_plan(int M, int H, int I, bool bf16) { return plan_product(M, H, I, bf16, false, USE_STORE, PARTIAL_ROWS); }
+int64_t gated_ws_bytes(int M, int H, int I, bool bf16) {
+    if (M <= FEW_ROWS) return bf16 ? up((int64_t)M * I * 4, 256) : 0;
+    return up(down_plan(M, H, I, bf16).partial, 256);
+}
 
 template <class T>
 static void gated(const GatedArgs& g, hipStream_t s) {
-    constexpr bool F32 = sizeof(T) == 4;
+    constexpr bool BF16 = sizeof(T) == 2;
+    if (g.M <= FEW_ROWS) {
+        few<T>(g, s);
+        return;
+    }
     TileArgs a{};
     a.A = g.X;
     a.lda = (int)g.ldx;
@@ -161,7 +387,7 @@ static void gated(const GatedArgs& g, hipStream_t s) {
     a.h = g.h;
     a.gu = g.gu;
     a.act = g.act;
-    product<T, false, false, USE_GATE>(a, pick_tile(g.M, 2 * (int64_t)g.I, F32, false), s);
+    product<T, false, false, USE_GATE>(a, plan_product(g.M, g.I, g.H, BF16, false, USE_GATE, 0), s);
     a.A = g.h;
     a.lda = g.I;
     a.B = g.Wd;
@@ -171,40 +397,44 @@ static void gated(const GatedArgs& g, hipStream_t s) {
     a.N = g.H;
     a.K = g.I;
     a.bias = g.bd;
-    product<T, false, false, USE_STORE>(a, pick_tile(g.M, g.H, F32, false), s);
+    stored_product<T, false, false>(a, down_plan(g.M, g.H, g.I, BF16), static_cast<float*>(g.ws), s);
 }
 
-template <class T>
-static void weight_gradient(TileArgs a, const SplitPlan& w, float* partial, void* out, hipStream_t s) {
-    a.splits = w.splits;
-    a.kt_split = w.kt;
-    a.ldc = a.N;
-    a.bias = nullptr;
-    if (w.splits == 1) {
-        a.C = out;
-        product<T, true, true, USE_STORE>(a, w.tile, s);
-        return;
-    }
-    a.C = partial;
-    product<T, true, true, USE_PARTIAL>(a, w.tile, s);
-    const int64_t n = (int64_t)a.M * a.N;
-    hipLaunchKernelGGL((sum_parts_kernel<T>), dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, s, partial, w.splits, n, static_cast<T*>(out));
+// The backward's workspace: [dg du], its column sums by row blocks, partial
+// sums of one product at a time, and partial column sums.
+struct BwdSpace {
+    int64_t colsum, partial, cols, bytes;
+    Plan slopes, dx, wgu, wd;
+};
+static BwdSpace bwd_space(int M, int H, int I, bool bf16) {
+    BwdSpace w;
+    const int64_t I2 = 2 * (int64_t)I;
+    w.slopes = plan_product(M, I, H, bf16, false, USE_SLOPES, 0);
+    w.dx = plan_product(M, H, I2, bf16, false, USE_STORE, PARTIAL_ROWS);
+    w.wgu = plan_product(I2, H, M, bf16, true, USE_STORE, PARTIAL_WEIGHTS);
+    w.wd = plan_product(H, I, M, bf16, true, USE_STORE, PARTIAL_WEIGHTS);
+    const TileShape& t = kTiles[w.slopes.tile];
+    w.colsum = up(M * I2 * (bf16 ? 2 : 4), 256);
+    w.partial = w.colsum + up(((int64_t)M + t.bm - 1) / t.bm * t.waves_m * I2 * 4, 256);
+    w.cols = w.partial + up(std::max({w.dx.partial, w.wgu.partial, w.wd.partial}), 256);
+    w.bytes = w.cols + up(64 * std::max<int64_t>(I2, H) * 4, 256);
+    return w;
 }
+int64_t gated_bwd_ws_bytes(int M, int H, int I, bool bf16) { return bwd_space(M, H, I, bf16).bytes; }
 
 template <class T>
 static void gated_bwd(const GatedArgs& g, hipStream_t s) {
-    constexpr bool F32 = sizeof(T) == 4;
-    const BwdSpace w = bwd_space(g.M, g.H, g.I, !F32);
-    char* const ws = static_cast<char*>(g.ws);
     const int64_t I2 = 2 * (int64_t)g.I;
     if (g.M == 0) {   // sums over no rows
-        const int64_t es = sizeof(T) / 2;   // in 16-bit halves of words
-        if (g.dWgu) launch_zero_words(g.dWgu, I2 * g.H * es / 2, s);
-        if (g.dWd) launch_zero_words(g.dWd, (int64_t)g.H * g.I * es / 2, s);
+        const int64_t words = sizeof(T) * g.H * (int64_t)g.I / 4;
+        if (g.dWgu) launch_zero_words(g.dWgu, 2 * words, s);
+        if (g.dWd) launch_zero_words(g.dWd, words, s);
         if (g.dbgu) launch_zero_words(g.dbgu, I2, s);
         if (g.dbd) launch_zero_words(g.dbd, g.H, s);
         return;
     }
+    const BwdSpace w = bwd_space(g.M, g.H, g.I, sizeof(T) == 2);
+    char* const ws = static_cast<char*>(g.ws);
     float* const colsum = reinterpret_cast<float*>(ws + w.colsum);
     float* const partial = reinterpret_cast<float*>(ws + w.partial);
     float* const cols = reinterpret_cast<float*>(ws + w.cols);
@@ -222,10 +452,10 @@ static void gated_bwd(const GatedArgs& g, hipStream_t s) {
         a.gu = g.gu;
         a.dgu = ws;
         a.colsum = g.dbgu ? colsum : nullptr;
-        product<T, false, true, USE_SLOPES>(a, w.slopes_tile, s);
+        product<T, false, true, USE_SLOPES>(a, w.slopes, s);
         if (g.dbgu) {
-            const int bm = w.slopes_tile == 0 ? 256 : (w.slopes_tile == 1 ? 128 : 64);
-            sum_rows<float>(colsum, I2, (g.M + (int64_t)bm - 1) / bm * 2, (int)I2, cols, g.dbgu, s);
+            const TileShape& t = kTiles[w.slopes.tile];
+            sum_rows<float>(colsum, I2, ((int64_t)g.M + t.bm - 1) / t.bm * t.waves_m, (int)I2, cols, g.dbgu, s);
         }
     }
     if (g.dbd) sum_rows<T>(static_cast<const T*>(g.dY), g.lddy, g.M, g.H, cols, g.dbd, s);
@@ -239,7 +469,7 @@ static void gated_bwd(const GatedArgs& g, hipStream_t s) {
         a.M = g.M;
         a.N = g.H;
         a.K = (int)I2;
-        product<T, false, true, USE_STORE>(a, pick_tile(g.M, g.H, F32, false), s);
+        stored_product<T, false, true>(a, w.dx, partial, s);
     }
     a.K = g.M;
     if (g.dWgu) {
@@ -247,18 +477,22 @@ static void gated_bwd(const GatedArgs& g, hipStream_t s) {
         a.lda = (int)I2;
         a.B = g.X;
         a.ldb = (int)g.ldx;
+        a.C = g.dWgu;
+        a.ldc = g.H;
         a.M = (int)I2;
         a.N = g.H;
-        weight_gradient<T>(a, w.wgu, partial, g.dWgu, s);
+        stored_product<T, true, true>(a, w.wgu, partial, s);
     }
     if (g.dWd) {
         a.A = g.dY;
         a.lda = (int)g.lddy;
         a.B = g.h;
         a.ldb = g.I;
+        a.C = g.dWd;
+        a.ldc = g.I;
         a.M = g.H;
         a.N = g.I;
-        weight_gradient<T>(a, w.wd, partial, g.dWd, s);
+        stored_product<T, true, true>(a, w.wd, partial, s);
     }
 }
 

@@ -31,6 +31,8 @@ int check_ffn(int32_t M, int32_t H, int32_t I, int32_t dtype) {
     if (M < 0 || H <= 0 || I <= 0 || H % 8 || I % 8 || H > kFfnMaxDim || I > kFfnMaxDim)
         return fail(EBH_ERR_INVALID_ARG, "bad FFN shape: M %d, H %d, I %d (H and I multiples of 8, at most %d)", M, H, I,
                     kFfnMaxDim);
+    if (2 * (int64_t)H * I * (int64_t)element(dtype) >= 0xFFFF0000ll)   // 32-bit offsets within the weights
+        return fail(EBH_ERR_INVALID_ARG, "FFN weights too large: 2 H I = %lld elements", 2 * (long long)H * I);
     return EBH_OK;
 }
 

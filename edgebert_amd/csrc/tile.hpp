@@ -40,8 +40,9 @@ struct TileArgs {
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ float logistic(float x) { return __builtin_amdgcn_rcpf(1.0f + fast_exp(-x)); }
 
-// Within 30 of 0, where every activation and slope has long reached its limit; NaN stays NaN.
-__device__ __forceinline__ float within_30(float g) { return g > 30.0f ? 30.0f : (g < -30.0f ? -30.0f : g); }
+// Within L of 0; NaN stays NaN.
+template <int L>
+__device__ __forceinline__ float within(float g) { return g > (float)L ? (float)L : (g < -(float)L ? -(float)L : g); }
 
 // The normal distribution function by formula 7.1.26 of Abramowitz and Stegun
 // (erf to 1.5e-7, here 0.75e-7, little over fp32's own half step at 1):
@@ -49,7 +50,7 @@ __device__ __forceinline__ float within_30(float g) { return g > 30.0f ? 30.0f :
 // No branches, no difference of near numbers for g < 0, and the exponential is
 // the one the derivative needs: e = e^(-g^2 / 2).
 __device__ __forceinline__ float normal_cdf(float g, float& e) {
-    const float m = fabsf(within_30(g));          // e^(-450) is 0
+    const float m = fabsf(within<30>(g));          // e^(-450) is 0
     e = fast_exp(-0.5f * m * m);
     const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, m, 1.0f));
     const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
@@ -70,25 +71,26 @@ __device__ __forceinline__ float act_of(float g) {
 // a = act(g), d = act'(g).
 template <int ACT>
 __device__ __forceinline__ void act_and_slope(float g, float& a, float& d) {
+    // x s(v) with s the logistic function: s = 1 / (1 + e), 1 - s = e s with e =
+    // e^(-v), no difference of near numbers.  v is held where e is finite; s has
+    // long reached its limit there, and g^2 stays in range.
     if constexpr (ACT == 0) {
-        // 1 - s as the logistic function of -g: no difference of near numbers
-        const float s = logistic(g);
+        const float e = fast_exp(-within<80>(g));
+        const float s = __builtin_amdgcn_rcpf(1.0f + e);
         a = g * s;
-        d = fmaf(a, logistic(-g), s);
+        d = fmaf(a, e * s, s);
     } else if constexpr (ACT == 1) {
-        // g s(2 u): s + g s(2 u) s(-2 u) 2 u'.  Past |g| = 30 one of the two is 0,
-        // and g^2 could pass the range
-        const float c = within_30(g);
-        const float u2 = 2.0f * 0.7978845608f * c * fmaf(0.044715f * c, c, 1.0f);
-        const float du2 = 2.0f * 0.7978845608f * fmaf(3.0f * 0.044715f * c, c, 1.0f);
-        const float s = logistic(u2);
+        const float c = within<10>(g), c2 = c * c;     // v = 2 u = 87 at 10
+        const float k = 2.0f * 0.7978845608f;
+        const float e = fast_exp(-(c * fmaf(k * 0.044715f, c2, k)));
+        const float s = __builtin_amdgcn_rcpf(1.0f + e);
         a = g * s;
-        d = fmaf(c * s * logistic(-u2), du2, s);
+        d = fmaf(c * s * (e * s), fmaf(3.0f * k * 0.044715f, c2, k), s);
     } else {
         float e;
         const float p = normal_cdf(g, e);
         a = g * p;
-        d = fmaf(within_30(g), 0.3989422804014327f * e, p);
+        d = fmaf(within<30>(g), 0.3989422804014327f * e, p);
     }
 }
 
@@ -125,10 +127,10 @@ __device__ __forceinline__ void act_grads(int act, const float* dh, float* g, fl
 }
 
 // ---------------------------------------------------------------------------
-// A tile's operands.  A k-tile is 128 bytes of k (64 bf16, 32 fp32) of BM rows of
-// A and BN of B, in LDS as it comes from memory, in 16-byte chunks that direct
+// A tile's operands.  A k-tile is KB bytes of k (128: 64 bf16, 32 fp32; or 64) of BM
+// rows of A and BN of B, in LDS as it comes from memory, in 16-byte chunks that direct
 // loads put where the fragment reads find them without bank conflicts:
-//  - k contiguous: rows of 8 chunks, chunk c of row r at c ^ chunk_swizzle16(r);
+//  - k contiguous: rows of KB / 16 chunks, chunk c of row r at c ^ chunk_swizzle16(r);
 //    a lane's operand is one 16-byte read;
 //  - k strided: rows of k, in units of 16 columns (32 bytes of bf16, 64 of
 //    fp32), unit b of row k at b ^ f(k).  bf16 operands come from
@@ -138,34 +140,41 @@ __device__ __forceinline__ void act_grads(int act, const float* dh, float* g, fl
 //    with f(k) = (k & 3) + 4 ((k >> 3) & 1).  fp32 operands are four reads of a
 //    word, at rows 4 q + e: f(k) = (k >> 2) & 3.
 // Lane (r, q) = (lane % 16, lane / 16) of a fragment holds row r of 16 and, of a
-// slice of half a k-tile, bf16 k = 8 q .. 8 q + 7, fp32 k = 4 q .. 4 q + 3 (one
+// slice of 64 bytes of k, bf16 k = 8 q .. 8 q + 7, fp32 k = 4 q .. 4 q + 3 (one
 // for each of four v_mfma_f32_16x16x4_f32).
 // ---------------------------------------------------------------------------
 constexpr uint32_t TILE_OUT = 0xFFFFFFE0u;    // an offset past every operand's k-tile
 constexpr uint32_t TILE_NONE = 0x80000000u;   // past every output's rows in a tile, and block steps above it too
 
-template <class T, bool STRIDED, int ROWS, int NT>
+// Columns of a row of k in LDS: 192 bf16 are a row and a half of all banks, and take two.
+template <bool STRIDED, int ROWS>
+constexpr int tile_pitch() { return STRIDED && ROWS == 192 ? 256 : ROWS; }
+
+template <class T, bool STRIDED, int ROWS, int KB, int NT, bool PLAIN>
 struct TileLoader {
-    static constexpr int ES = sizeof(T), KT = 128 / ES, CE = 16 / ES;
-    static constexpr int L = ROWS * 8 / NT;          // loads per thread and k-tile
-    static constexpr int CPR = STRIDED ? ROWS * ES / 16 : 8;   // chunks per row in LDS
+    static constexpr int ES = sizeof(T), KT = KB / ES, CE = 16 / ES, PITCH = tile_pitch<STRIDED, ROWS>();
+    static constexpr int L = PITCH * (KB / 16) / NT;   // loads per thread and k-tile
+    static constexpr int CPR = STRIDED ? PITCH * ES / 16 : KB / 16;   // chunks per row in LDS
     static constexpr int CU = ES;                    // chunks per unit of 16 columns
     static constexpr int RPL = NT / CPR;             // rows a pass of loads covers
-    static_assert(L * NT == ROWS * 8 && RPL >= 1 && (STRIDED || RPL % 32 == 0) && NT % CPR == 0, "passes of whole rows");
+    static_assert(L * NT == PITCH * (KB / 16) && RPL >= 1 && (STRIDED || RPL % 32 == 0) && NT % CPR == 0, "passes of whole rows");
 
     static __device__ __forceinline__ int f(int k) {
         return ES == 2 ? (k & 3) + 4 * ((k >> 3) & 1) : (k >> 2) & 3;
     }
 
     uint32_t ldb;         // bytes between rows
+    // A pass's chunks lie a fixed number of rows behind the one before's, except where
+    // the swizzle (fp32, strided) or the panel's rows (the gate's) go another way
+    static constexpr bool EVEN = PLAIN && PITCH == ROWS && (!STRIDED || (ES == 2 && RPL % 16 == 0));
     uint32_t voff[L];     // this thread's chunks, from the k-tile's start
     int chunk;            // k contiguous: the chunk's place in k
     uint64_t base;        // of the next k-tile to load
-    int64_t size;         // k contiguous: bytes from there to the panel's end
+    uint32_t size;        // k contiguous: bytes from there to the panel's end
     int left;             // k from there to the end
-    int cols;             // k strided: columns from the panel's first to the operand's last
+    uint32_t last;        // k strided: bytes of a row from the panel's first column to the operand's last
 
-    // rows_of(r): the row of the operand's panel that goes to row r in LDS.
+    // row_of(r): the row of the operand's panel that goes to row r in LDS.
     template <class F>
     __device__ __forceinline__ void init(int64_t ld, int tid, F&& row_of) {
         ldb = (uint32_t)(ld * ES);
@@ -174,9 +183,10 @@ struct TileLoader {
         for (int i = 0; i < L; ++i) {
             const int r = tid / CPR + i * RPL, slot = tid % CPR;
             if constexpr (STRIDED) {
-                voff[i] = (uint32_t)r * ldb + 16 * (slot ^ (CU * f(r)));
+                const int c = slot ^ (CU * f(r));
+                voff[i] = c < ROWS / CE ? (uint32_t)r * ldb + 16 * c : TILE_NONE;
             } else {
-                chunk = slot ^ chunk_swizzle16<8>(r);     // the same for all: passes are multiples of 16 rows
+                chunk = slot ^ chunk_swizzle16<CPR>(r);     // the same for all: passes are multiples of 16 rows
                 voff[i] = (uint32_t)row_of(r) * ldb + 16 * chunk;
             }
         }
@@ -186,50 +196,56 @@ struct TileLoader {
         left = (int)(K - k0);
         if constexpr (STRIDED) {
             base = uniform_u64(static_cast<const char*>(p) + (k0 * ld + r0) * ES);
-            cols = (int)(rows - r0);
+            last = (uint32_t)(rows - r0) * ES;
         } else {
             base = uniform_u64(static_cast<const char*>(p) + (r0 * ld + k0) * ES);
-            size = ((rows - r0 - 1) * ld + K - k0) * ES;
-            const int64_t most = 0xFFFF0000;              // offsets within a tile stay below it
-            if (size > most) size = most;
+            size = left > 0 ? (uint32_t)((rows - r0 - 1) * ld + left) * ES : 0u;   // less than 2^32: layer_ops.cpp
         }
     }
-    // The next k-tile into LDS at `lds` (this wave's part of the stage).
-    __device__ __forceinline__ void issue(uint32_t lds) {
+    // The next k-tile's loads, one at a time, into LDS at `lds` (this wave's part of the stage).
+    __device__ __forceinline__ void load(int i, uint32_t lds) const {
         uint32_t bytes;
-        if constexpr (STRIDED) bytes = left > 0 ? (uint32_t)(min(left, KT) - 1) * ldb + (uint32_t)cols * ES : 0u;
-        else bytes = left > 0 && size > 0 ? (uint32_t)size : 0u;
-        const g16_v4i rsrc = {(int)(uint32_t)base, (int)((uint32_t)(base >> 32) & 0xffffu), __builtin_amdgcn_readfirstlane((int)bytes),
-                              G16_RSRC_WORD3};
+        if constexpr (STRIDED) bytes = left > 0 ? (uint32_t)(min(left, KT) - 1) * ldb + last : 0u;
+        else bytes = left > 0 ? size : 0u;
+        const g16_v4i rsrc = {(int)(uint32_t)base, (int)((uint32_t)(base >> 32) & 0xffffu), (int)bytes, G16_RSRC_WORD3};
+        uint32_t v = EVEN ? voff[0] + i * RPL * ldb : voff[i];
         // k ends inside this k-tile: what lies behind it in a row is not zeros
-        const bool cut = !STRIDED && left < KT;
-        const bool out = cut && chunk * CE >= left;
-#pragma unroll
-        for (int i = 0; i < L; ++i) load_lds16_buf(rsrc, out ? TILE_OUT : voff[i], 0, lds + i * NT * 16);
+        if (!STRIDED && left < KT) v = chunk * CE >= left ? TILE_OUT : v;
+        asm volatile(
+            "s_mov_b32 m0, %2\n\t"
+            "s_nop 0\n\t"
+            "buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(v), "s"(rsrc), "s"(lds + i * NT * 16)
+            : "memory", "m0");
+    }
+    __device__ __forceinline__ void advance() {
         left -= KT;
         if constexpr (STRIDED) {
             base += (uint64_t)KT * ldb;
         } else {
-            base += 128;
-            size -= 128;
+            base += KB;
+            size -= KB;
         }
     }
 };
 
-template <class T, bool STRIDED, int ROWS>
+template <class T, bool STRIDED, int ROWS, int KB>
 struct TileReader {
-    static constexpr int ES = sizeof(T), RB = ROWS * ES;
+    static constexpr int ES = sizeof(T), RB = tile_pitch<STRIDED, ROWS>() * ES;
     uint32_t off;         // this lane's place
     __device__ __forceinline__ void init(int lane) {
         const int r = lane & 15, q = lane >> 4;
-        if constexpr (!STRIDED) off = r * 128 + 16 * (q ^ chunk_swizzle16<8>(r));
+        if constexpr (!STRIDED) off = r * KB + 16 * (q ^ chunk_swizzle16<KB / 16>(r));
         else if constexpr (ES == 2) off = (8 * q + (r >> 2)) * RB + 32 * ((r >> 2) + 4 * (q & 1)) + 8 * (r & 3);
         else off = 4 * q * RB + 64 * q + 4 * r;
+    }
+    // Strided: the blocks' places are formed anew in each k-tile, not held
+    __device__ __forceinline__ void renew() {
+        if constexpr (STRIDED) asm volatile("" : "+v"(off));
     }
     // The operand of block b (16 rows or columns) and slice s, `st` the stage's LDS address.
     __device__ __forceinline__ g16_v4f read(const char* st, int b, int s) const {
         if constexpr (!STRIDED) {
-            return *reinterpret_cast<const g16_v4f*>(st + (off ^ (64 * s)) + b * 2048);
+            return *reinterpret_cast<const g16_v4f*>(st + (off ^ (64 * s)) + b * 16 * KB);
         } else if constexpr (ES == 2) {
             typedef short v4s __attribute__((ext_vector_type(4)));
             typedef short v8s __attribute__((ext_vector_type(8)));
@@ -245,47 +261,75 @@ struct TileReader {
     }
 };
 
-// Two neighbouring blocks' accumulators (lane (r, q): columns 4 q .. 4 q + 3 of
-// row r) as eight consecutive columns: the second and fourth 16 lanes of the
-// one change places with the first and third of the other.  Lane (r, q) then has
-// columns 16 (q % 2) + 8 (q / 2) .. + 7 of the 32.
-__device__ __forceinline__ void eight_columns(const g16_v4f& a, const g16_v4f& b, float* v) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(a[e]), __float_as_uint(b[e]), false, false);
-        v[e] = __uint_as_float(s[0]);
-        v[4 + e] = __uint_as_float(s[1]);
+// Two neighbouring blocks of a row, a lane's columns 4 q .. 4 q + 3 of each, as they
+// lie in memory.  bf16: 16 bytes a lane, columns 16 (q % 2) + 8 (q / 2) .. + 7 of the
+// 32: of the packed words, the second and fourth 16 lanes of the one block change
+// places with the first and third of the other.
+__device__ __forceinline__ u4v_t swap_blocks(const u4v_t& w) {
+    const auto s = __builtin_amdgcn_permlane16_swap(w[0], w[2], false, false);
+    const auto t = __builtin_amdgcn_permlane16_swap(w[1], w[3], false, false);
+    return u4v_t{s[0], t[0], s[1], t[1]};
+}
+__device__ __forceinline__ u4v_t words(const float* v) {
+    return u4v_t{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+}
+// ES: bytes of an element in memory; o: the lane's places (of both blocks, where they
+// are two).  AUX 2: non-temporal.
+template <int ES, int AUX = 0>
+__device__ __forceinline__ void put_blocks(const __amdgpu_buffer_rsrc_t& d, const uint32_t* o, uint32_t add, const float* a, const float* b) {
+    if constexpr (ES == 2) {
+        const u4v_t w = swap_blocks(u4v_t{pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3])});
+        __builtin_amdgcn_raw_buffer_store_b128(w, d, o[0] + add, 0, AUX);
+    } else {
+        __builtin_amdgcn_raw_buffer_store_b128(words(a), d, o[0] + add, 0, AUX);
+        __builtin_amdgcn_raw_buffer_store_b128(words(b), d, o[1] + add, 0, AUX);
     }
 }
-__device__ __forceinline__ u4v_t pack8(const float* v) {
-    return u4v_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
-}
-__device__ __forceinline__ void unpack8(const u4v_t& w, float* v) {
+template <int ES>
+struct RawBlocks {
+    u4v_t w[ES / 2];
+    __device__ __forceinline__ void load(const __amdgpu_buffer_rsrc_t& d, const uint32_t* o, uint32_t add) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        v[2 * e] = __uint_as_float(w[e] << 16);
-        v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+        for (int k = 0; k < ES / 2; ++k) w[k] = __builtin_amdgcn_raw_buffer_load_b128(d, o[k] + add, 0, 0);
     }
-}
+    __device__ __forceinline__ void values(float* a, float* b) const {
+        if constexpr (ES == 2) {
+            const u4v_t v = swap_blocks(w[0]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                a[2 * e] = __uint_as_float(v[e] << 16);
+                a[2 * e + 1] = __uint_as_float(v[e] & 0xffff0000u);
+                b[2 * e] = __uint_as_float(v[2 + e] << 16);
+                b[2 * e + 1] = __uint_as_float(v[2 + e] & 0xffff0000u);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                a[e] = __uint_as_float(w[0][e]);
+                b[e] = __uint_as_float(w[ES / 2 - 1][e]);
+            }
+        }
+    }
+};
 
 // A persistent grid walks the work items (C tiles, N-fastest, times the ranges of
 // k).  The k-tiles of a workgroup's items are one stream: the next one's loads
 // are in flight while a tile is finished.  A k-tile's last MFMAs run after the
 // next one's barrier (two sets of B fragments, so k-tiles come in pairs; one
 // past the end of k is zeros).
-template <class T, bool AKS, bool BKS, int BM, int BN, int WAVES_M, int WAVES_N, int NS, int USE>
+template <class T, bool AKS, bool BKS, int BM, int BN, int WAVES_M, int WAVES_N, int KB, int NS, int USE>
 __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
-    constexpr int NW = WAVES_M * WAVES_N, NT = 64 * NW, ES = sizeof(T), KT = 128 / ES;
+    constexpr int NW = WAVES_M * WAVES_N, NT = 64 * NW, ES = sizeof(T), KT = KB / ES, SL = KB / 64;
     constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, FM = WM / 16, FN = WN / 16;
-    static_assert(FM * 16 == WM && WN == 64 && FN == 4, "waves of 64 columns");
+    static_assert(FM * 16 == WM && FN * 16 == WN && FN % (USE == USE_GATE ? 4 : 2) == 0, "pairs of blocks");
     constexpr int SB = FM >= 8 ? 2 : 1, STEPS = FM / SB;
     static_assert(STEPS % 2 == 0, "steps alternate between two A sets");
-    constexpr bool WIDE = ES == 2 && USE != USE_PARTIAL;   // eight bf16 columns a lane, else four fp32 ones
-    constexpr int G = WIDE ? 2 : 4;                        // groups of columns a lane has in 64
+    constexpr int OS = USE == USE_PARTIAL ? 4 : ES;        // bytes of a stored element
+    constexpr int FC = USE == USE_GATE ? FN / 2 : FN;      // blocks of a wave's columns of C
     constexpr int BNC = USE == USE_GATE ? BN / 2 : BN;     // columns of C in a tile
-    constexpr int ST_A = BM * 128, ST_B = BN * 128, B_OFF = NS * ST_A;
-    constexpr int NLD = (BM + BN) * 8 / NT;                // loads per thread and k-tile
-    constexpr int NSTO = FM * G / (USE == USE_GATE ? 2 : 1);   // stores per thread and tile, at least
+    constexpr int ST_A = BM * KB, ST_B = tile_pitch<BKS, BN>() * KB, B_OFF = NS * ST_A;
+    constexpr int NLD = (ST_A + ST_B) / 16 / NT;                // loads per thread and k-tile
+    constexpr int NSTO = FM * FC * OS / 4;                 // stores per thread and tile, at least
 
     const int ntn = (p.N + BNC - 1) / BNC, ntiles = ((p.M + BM - 1) / BM) * ntn, nwork = ntiles * p.splits, nk = p.kt_split;
     // Workgroup b runs on XCD b % 8; each XCD's workgroups take consecutive items,
@@ -302,16 +346,21 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
     }
     const int my_tiles = u0 < uend ? (uend - u0 + ustep - 1) / ustep : 0;
     if (my_tiles == 0) return;   // uniform over the workgroup
+    // One workgroup a CU: neighbours in an XCD start 2,048 clocks apart, in four
+    // phases, or the whole chip would load, multiply and store in step (32,768
+    // rows, 768 -> 2 x 2,048: 250 -> 188 us; the slopes of it 193 -> 183 us)
+    if constexpr (NT == 512)
+        for (int w = (blockIdx.x >> 3) & 3; w > 0; --w) __builtin_amdgcn_s_sleep(32);
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WAVES_N, wn = wave % WAVES_N;
     const uint32_t lds0 = (uint32_t)(uintptr_t)smem + (uint32_t)wave * 1024;
 
-    TileLoader<T, AKS, BM, NT> la;
-    TileLoader<T, BKS, BN, NT> lb;
+    TileLoader<T, AKS, BM, KB, NT, true> la;
+    TileLoader<T, BKS, BN, KB, NT, USE != USE_GATE> lb;
     la.init(p.lda, tid, [](int r) { return r; });
-    // USE_GATE: each wave's 64 columns are 32 of the gate's and the same 32 of the other's
-    lb.init(p.ldb, tid, [&](int r) { return USE == USE_GATE ? (r >> 6) * 32 + (r & 31) + (r & 32 ? p.N : 0) : r; });
+    // USE_GATE: half of each wave's columns are the gate's, the others the same ones of the other projection
+    lb.init(p.ldb, tid, [&](int r) { return USE == USE_GATE ? r / WN * (WN / 2) + r % (WN / 2) + (r % WN < WN / 2 ? 0 : p.N) : r; });
     int lt = 0, lkt = 0, li = 0;   // the stream's next k-tile: its item, its place in it, its number
     auto item = [&](int t, int& m0, int& n0, int& split) __attribute__((always_inline)) {
         const int u = u0 + t * ustep;
@@ -327,11 +376,22 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
         la.at(p.A, p.lda, m0, AKS ? p.M : min(p.M, m0 + BM), k0, p.K);
         lb.at(p.B, p.ldb, n0, USE == USE_GATE ? 2 * (int64_t)p.N : (BKS ? p.N : min(p.N, n0 + BN)), k0, p.K);
     };
-    auto issue = [&]() __attribute__((always_inline)) {
+    // The next k-tile's loads n .. n + count - 1 of this thread, into the stage of its
+    // number, even or odd (k-tiles come in pairs) or by the count.
+    constexpr int LA = decltype(la)::L, LOADS = LA + decltype(lb)::L;
+    auto loads = [&](int n, int count, int par) __attribute__((always_inline)) {
         if (lt >= my_tiles) return;
-        const uint32_t st = li % NS;
-        la.issue(lds0 + st * ST_A);
-        lb.issue(lds0 + B_OFF + st * ST_B);
+        const uint32_t st = NS == 2 ? par : li % NS;
+#pragma unroll
+        for (int i = n; i < n + count && i < LOADS; ++i) {
+            if (i < LA) la.load(i, lds0 + st * ST_A);
+            else lb.load(i - LA, lds0 + B_OFF + st * ST_B);
+        }
+    };
+    auto next = [&]() __attribute__((always_inline)) {
+        if (lt >= my_tiles) return;
+        la.advance();
+        lb.advance();
         ++li;
         if (++lkt == nk) {
             lkt = 0;
@@ -339,11 +399,11 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
         }
     };
 
-    TileReader<T, AKS, BM> ra;
-    TileReader<T, BKS, BN> rb;
+    TileReader<T, AKS, BM, KB> ra;
+    TileReader<T, BKS, BN, KB> rb;
     ra.init(lane);
     rb.init(lane);
-    g16_v4f acc[FM][FN], af[2][SB][2], bf[2][FN][2];
+    g16_v4f acc[FM][FN], af[2][SB][SL], bf[2][FN][SL];
     int it = 0;
     // The stream's k-tile `it` is in LDS, and everyone is done with the one before.
     // Issued behind its loads: at most those of the k-tiles between, and a tile's stores.
@@ -362,13 +422,18 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
         }
         lds_barrier();
     };
-    auto mfma_step = [&](int s, int as, int bs) __attribute__((always_inline)) {
+    // One step's MFMAs.  A load holds up its wave until the CU's address unit has
+    // taken it, 16 clocks for each of the workgroup's waves: they go out one by one
+    // between the MFMAs, in the first half of a k-tile's slots (one after every
+    // FN); two workgroups a CU do with A's and B's in one go each.
+    constexpr int SLOTS = SB * SL, PER = NT == 256 ? LA : (2 * LOADS + STEPS * SLOTS - 1) / (STEPS * SLOTS);
+    auto mfma_step = [&](int s, int as, int bs, int slot, int par) __attribute__((always_inline)) {
 #pragma unroll
-        for (int sl = 0; sl < 2; ++sl)
+        for (int sl = 0; sl < SL; ++sl)
 #pragma unroll
-            for (int e = 0; e < (ES == 2 ? 1 : 4); ++e)
+            for (int i = 0; i < SB; ++i) {
 #pragma unroll
-                for (int i = 0; i < SB; ++i)
+                for (int e = 0; e < (ES == 2 ? 1 : 4); ++e)
 #pragma unroll
                     for (int j = 0; j < FN; ++j) {
                         g16_v4f& d = acc[s * SB + i][j];
@@ -378,185 +443,205 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
                         else
                             d = __builtin_amdgcn_mfma_f32_16x16x4f32(bf[bs][j][sl][e], af[as][i][sl][e], d, 0, 0, 0);
                     }
+                if (slot >= 0 && slot * PER < LOADS) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    loads(slot * PER, PER, par);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                ++slot;
+            }
     };
     auto run_ktile = [&](auto set, bool first) __attribute__((always_inline)) {
         constexpr int P = decltype(set)::value;
-        const char *sa = smem + (it % NS) * ST_A, *sb = smem + B_OFF + (it % NS) * ST_B;
+        const int st = NS == 2 ? P : it % NS;
+        const char *sa = smem + st * ST_A, *sb = smem + B_OFF + st * ST_B;
         auto rd_a = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < SB; ++i)
 #pragma unroll
-                for (int sl = 0; sl < 2; ++sl) af[s & 1][i][sl] = ra.read(sa, wm * FM + s * SB + i, sl);
+                for (int sl = 0; sl < SL; ++sl) af[s & 1][i][sl] = ra.read(sa, wm * FM + s * SB + i, sl);
         };
+        ra.renew();
+        rb.renew();
         rd_a(0);
 #pragma unroll
         for (int j = 0; j < FN; ++j)
 #pragma unroll
-            for (int sl = 0; sl < 2; ++sl) bf[P][j][sl] = rb.read(sb, wn * FN + j, sl);
-        if (!first) mfma_step(STEPS - 1, 1, P ^ 1);   // the previous k-tile's last step
+            for (int sl = 0; sl < SL; ++sl) bf[P][j][sl] = rb.read(sb, wn * FN + j, sl);
+        __builtin_amdgcn_sched_barrier(0);            // reads stay ahead of the MFMAs that hide them
+        constexpr int par = NS == 2 ? P ^ 1 : 0;
+        if (!first) mfma_step(STEPS - 1, 1, P ^ 1, 0, par);   // the previous k-tile's last step
+        else loads(0, SLOTS * PER, par);
 #pragma unroll
         for (int s = 0; s + 1 < STEPS; ++s) {
-            if (s == 0) issue();
             rd_a(s + 1);
-            mfma_step(s, s & 1, P);
+            __builtin_amdgcn_sched_barrier(0);
+            mfma_step(s, s & 1, P, (s + 1) * SLOTS, par);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        next();
         ++it;
     };
 
     auto finish = [&](int t) __attribute__((always_inline)) {
         int m0, n0, split;
         item(t, m0, n0, split);
+        // What only this part reads of the arguments (the kernel's only one, at its
+        // arguments' start) comes from memory now: held across the k-loop it would
+        // spill scalar registers.
+        typedef const __attribute__((address_space(4))) TileArgs* Args;
+        Args ep = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(ep));
+        const float* const biases = ep->bias;
+        const int I = ep->I, act = ep->act;
         const int wrow = m0 + wm * WM;
         int el = lane;
         asm volatile("" : "+v"(el));   // formed here, not held across the k-loop
         const int r = el & 15, q = el >> 4;
-        // Block pair or block g of the wave's columns: this lane's first column of C
-        auto col = [&](int g) __attribute__((always_inline)) {
-            return n0 + (USE == USE_GATE ? wn * 32 : wn * WN) + (WIDE ? 32 * g + 16 * (q & 1) + 8 * (q >> 1) : 16 * g + 4 * q);
-        };
-        constexpr int V = WIDE ? 8 : 4;
-        auto values = [&](int i, int g, float* v) __attribute__((always_inline)) {
-            if constexpr (WIDE) {
-                eight_columns(acc[i][2 * g], acc[i][2 * g + 1], v);
+        const int cbase = n0 + wn * FC * 16;          // the wave's first column of C
+        auto col = [&](int j) __attribute__((always_inline)) { return cbase + 16 * j + 4 * q; };   // the lane's of block j
+        // The lane's places of blocks 2 jp and 2 jp + 1 in its row r, rows `bytes` apart
+        // (N is a multiple of 8: 8 or 4 columns are in or out together)
+        auto places = [&](int jp, int bytes, uint32_t* o) __attribute__((always_inline)) {
+            const int w = cbase + 32 * jp + 16 * (q & 1) + 8 * (q >> 1);
+            if constexpr (OS == 2) {
+                o[0] = w < p.N ? (uint32_t)(r * bytes + w * 2) : TILE_NONE;
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[i][g][e];
+                for (int b = 0; b < 2; ++b) o[b] = col(2 * jp + b) < p.N ? (uint32_t)(r * bytes + col(2 * jp + b) * 4) : TILE_NONE;
             }
         };
-        // The wave's rows of a matrix, and a lane's place in block i's (less than 2^31
-        // from the first: TILE_NONE is past every row's)
-        auto rows = [&](const void* base, int64_t ld, int es) __attribute__((always_inline)) {
+        // The wave's rows of a matrix; a lane's places in them are less than 2^31 from
+        // the first, and TILE_NONE is past them
+        auto rows = [&](const void* base, int bytes) __attribute__((always_inline)) {
             const int left = __builtin_amdgcn_readfirstlane(min(p.M - wrow, WM));
-            return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(base) + (int64_t)wrow * ld * es),
-                                                     (short)0, (left > 0 ? left : 0) * (int)(ld * es), G16_RSRC_WORD3);
+            return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(base) + (int64_t)wrow * bytes),
+                                                     (short)0, (left > 0 ? left : 0) * bytes, G16_RSRC_WORD3);
         };
-        auto put = [&](const __amdgpu_buffer_rsrc_t& d, uint32_t off, const float* v) __attribute__((always_inline)) {
-            if constexpr (WIDE) __builtin_amdgcn_raw_buffer_store_b128(pack8(v), d, off, 0, 0);
-            else
-                __builtin_amdgcn_raw_buffer_store_b128(
-                    u4v_t{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])}, d, off, 0, 0);
-        };
-        auto unpack = [&](const u4v_t& w, float* v) __attribute__((always_inline)) {
-            if constexpr (WIDE) {
-                unpack8(w, v);
-            } else {
+        auto bias = [&](int j, const float* from, float* v) __attribute__((always_inline)) {
+            const bool in = from && col(j) < p.N;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(w[e]);
-            }
+            for (int e = 0; e < 4; ++e) v[e] = in ? from[col(j) + e] : 0.0f;
         };
-        constexpr int OS = USE == USE_PARTIAL ? 4 : ES;      // bytes of a stored element
+        // Rows outermost: a row's neighbouring pairs are stored one after the other, whole lines.
         if constexpr (USE == USE_STORE || USE == USE_PARTIAL) {
-            char* const c = static_cast<char*>(p.C) + (USE == USE_PARTIAL ? (int64_t)split * p.M * p.ldc * 4 : 0);
-            float b[G][V];
-            uint32_t off[G];
+            int bytes = ep->ldc * OS;
+            asm volatile("" : "+s"(bytes));   // its multiples are formed here, not held
+            const auto d = rows(static_cast<char*>(ep->C) + (USE == USE_PARTIAL ? (int64_t)split * p.M * bytes : 0), bytes);
+            float bv[FN][4];
+            uint32_t o[FN / 2][2];
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-                const int n = col(g);
-                off[g] = n < p.N ? (uint32_t)(r * p.ldc * OS + n * OS) : TILE_NONE;
+            for (int j = 0; j < FN; ++j)
+                if (USE == USE_STORE) bias(j, biases, bv[j]);
 #pragma unroll
-                for (int e = 0; e < V; ++e) b[g][e] = USE == USE_STORE && p.bias && n < p.N ? p.bias[n + e] : 0.0f;
-            }
-            const auto d = rows(c, p.ldc, OS);
-            int step = 16 * p.ldc * OS;
-            asm volatile("" : "+s"(step));   // its multiples are formed here, not held
+            for (int jp = 0; jp < FN / 2; ++jp) places(jp, bytes, o[jp]);
 #pragma unroll
-            for (int i = 0; i < FM; ++i) {
+            for (int i = 0; i < FM; ++i)
 #pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    float v[V];
-                    values(i, g, v);
+                for (int jp = 0; jp < FN / 2; ++jp) {
+                    float v[2][4];
 #pragma unroll
-                    for (int e = 0; e < V; ++e) v[e] += b[g][e];
-                    put(d, off[g] + i * step, v);
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[b][e] = acc[i][2 * jp + b][e] + (USE == USE_STORE ? bv[2 * jp + b][e] : 0.0f);
+                    put_blocks<OS>(d, o[jp], i * 16 * bytes, v[0], v[1]);
                 }
-            }
         } else {
-            {
-                const int64_t I = p.I;
-                int row_h = p.I * ES;
-                asm volatile("" : "+s"(row_h));   // its multiples are formed here, not held
-                const int row_gu = 2 * row_h;
-                if constexpr (USE == USE_GATE) {
-                    const auto dh = rows(p.h, I, ES), dgu = rows(p.gu, 2 * I, ES);
+            void* const gu = ep->gu;
+            int row_h = I * ES;
+            asm volatile("" : "+s"(row_h));
+            const int row_gu = 2 * row_h;
+            uint32_t og[FC / 2][2];
 #pragma unroll
-                    for (int g = 0; g < G / 2; ++g) {
-                        const int n = col(g);
-                        const bool in = n < p.N;
-                        float bg[V], bu[V];
+            for (int jp = 0; jp < FC / 2; ++jp) places(jp, row_gu, og[jp]);
+            if constexpr (USE == USE_GATE) {
+                const auto dh = rows(ep->h, row_h), dgu = rows(gu, row_gu);
+                uint32_t oh[FC / 2][2];
 #pragma unroll
-                        for (int e = 0; e < V; ++e) {
-                            bg[e] = p.bias && in ? p.bias[n + e] : 0.0f;
-                            bu[e] = p.bias && in ? p.bias[I + n + e] : 0.0f;
-                        }
-                        uint32_t oh = in ? (uint32_t)(r * row_h + n * ES) : TILE_NONE;
-                        uint32_t og = in ? (uint32_t)(r * row_gu + n * ES) : TILE_NONE;
+                for (int jp = 0; jp < FC / 2; ++jp) places(jp, row_h, oh[jp]);
+                float bg[FC][4], bu[FC][4];
 #pragma unroll
-                        for (int i = 0; i < FM; ++i) {
-                            float gv[V], uv[V], hv[V];
-                            values(i, g, gv);
-                            values(i, G / 2 + g, uv);
+                for (int j = 0; j < FC; ++j) {
+                    bias(j, biases, bg[j]);
+                    bias(j, biases ? biases + I : nullptr, bu[j]);
+                }
 #pragma unroll
-                            for (int e = 0; e < V; ++e) {
-                                gv[e] += bg[e];
-                                uv[e] += bu[e];
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int jp = 0; jp < FC / 2; ++jp) {
+                        float g[2][4], u[2][4], hv[2][4];
+#pragma unroll
+                        for (int b = 0; b < 2; ++b)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                g[b][e] = acc[i][2 * jp + b][e] + bg[2 * jp + b][e];
+                                u[b][e] = acc[i][FC + 2 * jp + b][e] + bu[2 * jp + b][e];
                             }
-                            act_times<V>(p.act, gv, uv, hv);
-                            put(dh, oh, hv);
-                            if (p.gu) {
-                                put(dgu, og, gv);
-                                put(dgu, og + row_h, uv);
-                            }
-                            oh += 16 * row_h;
-                            og += 16 * row_gu;
+                        act_times<8>(act, g[0], u[0], hv[0]);
+                        put_blocks<ES>(dh, oh[jp], i * 16 * row_h, hv[0], hv[1]);
+                        if (gu) {   // not read before the backward pass: kept out of the caches
+                            put_blocks<ES, 2>(dgu, og[jp], i * 16 * row_gu, g[0], g[1]);
+                            put_blocks<ES, 2>(dgu, og[jp], i * 16 * row_gu + row_h, u[0], u[1]);
                         }
+                        __builtin_amdgcn_sched_barrier(0);   // one pair's values at a time in registers
                     }
-                } else {
-                    const auto src = rows(p.gu, 2 * I, ES), dst = rows(p.dgu, 2 * I, ES);
+            } else {
+                const auto src = rows(gu, row_gu), dst = rows(ep->dgu, row_gu);
+                constexpr int N = FM * FN / 2, AHEAD = N < 4 ? N : 4;   // pairs of blocks, and how many's g and u are on their way
+                float* const colsum = ep->colsum;
+                float cg[FN][4] = {}, cu[FN][4] = {};
+                RawBlocks<ES> raw[AHEAD][2];
+                // pair k, `rows16` rows of blocks on from where og has come to
+                auto load = [&](int k, int rows16) __attribute__((always_inline)) {
+                    raw[k % AHEAD][0].load(src, og[k % (FN / 2)], rows16 * 16 * row_gu);
+                    raw[k % AHEAD][1].load(src, og[k % (FN / 2)], rows16 * 16 * row_gu + row_h);
+                };
 #pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        const int n = col(g);
-                        uint32_t og = n < p.N ? (uint32_t)(r * row_gu + n * ES) : TILE_NONE;
-                        float cg[V] = {}, cu[V] = {};
-                        u4v_t raw[2][2];           // g and u of this block of rows and the next
-                        auto load = [&](int set, uint32_t at) __attribute__((always_inline)) {
-                            raw[set][0] = __builtin_amdgcn_raw_buffer_load_b128(src, at, 0, 0);
-                            raw[set][1] = __builtin_amdgcn_raw_buffer_load_b128(src, at + row_h, 0, 0);
-                        };
-                        load(0, og);
+                for (int k = 0; k < AHEAD; ++k) load(k, k / (FN / 2));
 #pragma unroll
-                        for (int i = 0; i < FM; ++i) {
-                            float gv[V], uv[V], dh[V];
-                            if (i + 1 < FM) load((i + 1) & 1, og + 16 * row_gu);
-                            unpack(raw[i & 1][0], gv);
-                            unpack(raw[i & 1][1], uv);
-                            values(i, g, dh);
-                            act_grads<V>(p.act, dh, gv, uv);
+                for (int k = 0; k < N; ++k) {
+                    const int i = k / (FN / 2), jp = k % (FN / 2);
+                    float g[2][4], u[2][4], dh[2][4];
+                    raw[k % AHEAD][0].values(g[0], g[1]);
+                    raw[k % AHEAD][1].values(u[0], u[1]);
+                    if (k + AHEAD < N) load(k + AHEAD, (k + AHEAD) / (FN / 2) - i);
 #pragma unroll
-                            for (int e = 0; e < V; ++e) {
-                                cg[e] += gv[e];
-                                cu[e] += uv[e];
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) dh[b][e] = acc[i][2 * jp + b][e];
+                    act_grads<8>(act, dh[0], g[0], u[0]);
+                    if (colsum) {
+#pragma unroll
+                        for (int b = 0; b < 2; ++b)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                cg[2 * jp + b][e] += g[b][e];
+                                cu[2 * jp + b][e] += u[b][e];
                             }
-                            put(dst, og, gv);
-                            put(dst, og + row_h, uv);
-                            og += 16 * row_gu;
-                            __builtin_amdgcn_sched_barrier(0);   // keeps the loads one block ahead, not all at once
-                        }
-                        if (p.colsum) {
-                            // rows past the last are zeros: dh is, of operands that are
+                    }
+                    put_blocks<ES>(dst, og[jp], 0, g[0], g[1]);
+                    put_blocks<ES>(dst, og[jp], row_h, u[0], u[1]);
+                    og[jp][0] += 16 * row_gu;
+                    og[jp][1] += 16 * row_gu;
+                    __builtin_amdgcn_sched_barrier(0);   // keeps the loads so far ahead, not all of them
+                }
+                if (colsum) {
+                    // rows past the last are zeros: dh is, of operands that are
 #pragma unroll
-                            for (int e = 0; e < V; ++e)
+                    for (int j = 0; j < FN; ++j) {
 #pragma unroll
-                                for (int o = 1; o < 16; o <<= 1) {
-                                    cg[e] += __shfl_xor(cg[e], o);
-                                    cu[e] += __shfl_xor(cu[e], o);
-                                }
-                            if (r == 0 && n < p.N) {
-                                float* at = p.colsum + (int64_t)(m0 / BM * WAVES_M + wm) * 2 * I + n;
+                        for (int e = 0; e < 4; ++e)
 #pragma unroll
-                                for (int e = 0; e < V; ++e) {
-                                    at[e] = cg[e];
-                                    at[I + e] = cu[e];
-                                }
+                            for (int o = 1; o < 16; o <<= 1) {
+                                cg[j][e] += __shfl_xor(cg[j][e], o);
+                                cu[j][e] += __shfl_xor(cu[j][e], o);
+                            }
+                        if (r == 0 && col(j) < p.N) {
+                            float* at = colsum + (int64_t)(m0 / BM * WAVES_M + wm) * 2 * I + col(j);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                at[e] = cg[j][e];
+                                at[I + e] = cu[j][e];
                             }
                         }
                     }
@@ -567,7 +652,10 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
 
     cursors(0);
 #pragma unroll
-    for (int d = 0; d < NS - 1; ++d) issue();
+    for (int d = 0; d < NS - 1; ++d) {
+        loads(0, LOADS, d);
+        next();
+    }
     typedef std::integral_constant<int, 0> set0;
     typedef std::integral_constant<int, 1> set1;
     for (int t = 0; t < my_tiles; ++t) {
@@ -585,11 +673,12 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
             enter(false);
             run_ktile(set1{}, false);
         }
-        mfma_step(STEPS - 1, 1, 1);
+        mfma_step(STEPS - 1, 1, 1, -SLOTS, 0);
         finish(t);
     }
 }
 
-constexpr int tile_lds(int bm, int bn, int ns) { return (bm + bn) * 128 * ns; }
+template <bool BKS, int BM, int BN, int KB, int NS>
+constexpr int tile_lds() { return (BM + tile_pitch<BKS, BN>()) * KB * NS; }
 
 }  // namespace ebh

@@ -424,8 +424,14 @@ def check_ffn(env, M, H, I, act, bf16, bias, extra=0, keep=True):
     h64 = a * u
     th = a.abs() * tu + ta * (u.abs() + tu) + 2 * U * h64.abs()
     near(torch, h, h64, th + E * (h64.abs() + th), "h")
-    y64 = h.double() @ wd.T + (c["bd"].double() if bias else 0.0)    # of the h that was written
-    ty = product_tol(torch, h.double(), wd.T) + 2 * U * y64.abs()
+    bd = c["bd"].double() if bias else 0.0
+    if bf16 and M <= 64:
+        # of h before its rounding, as two bf16 (2^-17 of each value)
+        y64 = h64 @ wd.T + bd
+        ty = product_tol(torch, h64, wd.T, 2.0 ** -17) + th @ wd.T.abs() + 2 * U * y64.abs()
+    else:                                                            # of the h that was written
+        y64 = h.double() @ wd.T + bd
+        ty = product_tol(torch, h.double(), wd.T) + 2 * U * y64.abs()
     near(torch, y, y64, ty + E * (y64.abs() + ty), "y")
     return c
 

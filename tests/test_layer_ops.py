@@ -106,7 +106,7 @@ def ffn_bwd(**kw):
 
 
 SHAPES = [(dict(dtype=2), "unknown dtype"), (dict(M=-1), "shape"), (dict(H=0), "shape"), (dict(I=0), "shape"), (dict(H=60), "shape"),
-          (dict(I=68), "shape"), (dict(H=65544, ldx=65544), "shape"), (dict(I=65544), "shape"), (dict(act=3), "activation"),
+          (dict(I=68), "shape"), (dict(H=65544, ldx=65544), "shape"), (dict(I=65544), "shape"), (dict(H=32768, I=32768, ldx=32768), "too large"), (dict(act=3), "activation"),
           (dict(act=-1), "activation")]
 
 
