@@ -24,7 +24,7 @@ bool known_dtype(int32_t dtype) { return dtype == EBH_DTYPE_F32 || dtype == EBH_
 bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 uintptr_t element(int32_t dtype) { return dtype == EBH_DTYPE_BF16 ? 2 : 4; }
 
-constexpr int32_t kNormMaxH = 16384, kFfnMaxDim = 65536;
+constexpr int32_t kNormMaxH = 8192, kFfnMaxDim = 65536;
 
 int check_ffn(int32_t M, int32_t H, int32_t I, int32_t dtype) {
     if (!known_dtype(dtype)) return fail(EBH_ERR_INVALID_ARG, "unknown dtype %d", dtype);
@@ -59,7 +59,7 @@ int ebh_op_rope(const void* x, int64_t ldx, void* y, int64_t ldy, int32_t dtype,
                 int32_t transpose, void* stream) {
     if (!cfg) return fail(EBH_ERR_INVALID_ARG, "null rope config");
     if (!known_dtype(dtype)) return fail(EBH_ERR_INVALID_ARG, "unknown dtype %d", dtype);
-    if (T < 0 || n_heads <= 0 || head_dim <= 0 || head_dim > 1024 || (int64_t)n_heads * head_dim > (1 << 30))
+    if (T < 0 || n_heads <= 0 || n_heads > 65536 || head_dim <= 0 || head_dim > 1024)
         return fail(EBH_ERR_INVALID_ARG, "bad rope shape: T %d, %d heads of %d", T, n_heads, head_dim);
     const ebh_rope& c = *cfg;
     if (c.rot_dim < 2 || c.rot_dim % 2 || c.rot_dim > head_dim)

@@ -257,8 +257,8 @@ typedef struct ebh_rope {
  * k of a qkv row.  y may be x (ldy = ldx).  n_tokens (device, nullable): only the
  * first *n_tokens of the T rows are turned, the others not read nor written.
  * transpose != 0: the transposed map, angle -pos * f_i, which takes a
- * gradient of y to one of x.  Angles are formed in 64 bits.  head_dim <= 1024,
- * pointers aligned to their elements. */
+ * gradient of y to one of x.  Angles are formed in 64 bits.  n_heads <= 65536,
+ * head_dim <= 1024, pointers aligned to their elements. */
 EBH_API int ebh_op_rope(const void* x, int64_t ldx, void* y, int64_t ldy, int32_t dtype, const int32_t* pos,
                 const int32_t* n_tokens, int32_t T, int32_t n_heads, int32_t head_dim, const ebh_rope* cfg,
                 int32_t transpose, void* stream);
@@ -266,7 +266,7 @@ EBH_API int ebh_op_rope(const void* x, int64_t ldx, void* y, int64_t ldy, int32_
 /* Layer norm over rows x [rows, H]: y = (x - mean) rstd gamma + beta, rstd = 1 /
  * sqrt(var + eps), population variance; gamma and beta [H] may be NULL (1 and
  * 0).  mean and rstd [rows] (nullable) are written for the backward pass.  y
- * may be x (ldy = ldx).  H <= 16384, pointers aligned to their elements. */
+ * may be x (ldy = ldx).  H <= 8192, pointers aligned to their elements. */
 EBH_API int ebh_op_layer_norm_fwd(const void* x, int64_t ldx, int32_t dtype, const float* gamma, const float* beta,
                           int32_t rows, int32_t H, float eps, void* y, int64_t ldy, float* mean, float* rstd,
                           void* stream);

@@ -174,7 +174,7 @@ def test_rope_transpose_takes_gradients_back(env):
 # Layer norm
 # ---------------------------------------------------------------------------
 NORM_SHAPES = [(1, 1), (1, 8), (3, 5), (2, 64), (65, 384), (1061, 769), (257, 768), (33, 1024), (9, 1000), (50, 2048),
-               (17, 2050), (5, 4096), (3, 8192), (2, 16384), (2, 16383), (5000, 24), (3000, 128), (4, 300), (31, 6000)]
+               (17, 2050), (5, 4096), (3, 8192), (2, 8191), (2, 7000), (5000, 24), (3000, 128), (4, 300), (31, 6000)]
 
 
 def norm_case(torch, rows, H, bf16, seed, offset=0.5, affine=True):
