@@ -98,10 +98,10 @@ struct TileTime {
     float launch, full, epi, one;
 };
 static const TileTime kTimes[2][4][TILES] = {   // bf16, fp32; by Use
-    {{{0.0f, 1.333f, 8.7f, 0}, {0.0f, 1.113f, 7.0f, 0}, {0.0f, 0.826f, 6.6f, 0.639f}, {4.2f, 0.629f, 1.3f, 0.434f}},
-     {{1.8f, 1.373f, 11.0f, 0}, {3.3f, 1.165f, 7.7f, 0}, {2.6f, 0.882f, 5.0f, 0.647f}, {3.7f, 0.619f, 2.2f, 0.412f}},
-     {{2.9f, 1.453f, 5.3f, 0}, {}, {3.5f, 1.086f, 0.6f, 0.646f}, {2.8f, 0.907f, 0.0f, 0.614f}},
-     {{0.0f, 1.337f, 20.5f, 0}, {}, {0.1f, 0.737f, 14.4f, 0.512f}, {2.2f, 0.729f, 4.8f, 0.504f}}},
+    {{{0.0f, 1.302f, 6.9f, 0}, {0.0f, 1.152f, 2.7f, 0}, {0.0f, 0.815f, 6.4f, 0.800f}, {3.9f, 0.634f, 0.0f, 0.429f}},
+     {{1.2f, 1.363f, 11.3f, 0}, {2.8f, 1.165f, 7.8f, 0}, {2.5f, 0.883f, 5.0f, 0.644f}, {3.7f, 0.602f, 2.2f, 0.403f}},
+     {{2.1f, 1.414f, 5.6f, 0}, {}, {3.5f, 1.082f, 0.4f, 0.617f}, {2.6f, 0.893f, 0.0f, 0.610f}},
+     {{0.0f, 1.282f, 20.5f, 0}, {}, {0.0f, 0.732f, 14.4f, 0.505f}, {2.1f, 0.743f, 4.7f, 0.511f}}},
     {{{}, {}, {5.5f, 7.39f, 4.0f, 3.963f}, {0.0f, 4.119f, 5.4f, 2.489f}},
      {{}, {}, {3.9f, 7.389f, 3.8f, 3.994f}, {3.8f, 4.013f, 1.8f, 2.374f}},
      {{}, {}, {0.0f, 6.766f, 10.4f, 3.953f}, {3.2f, 3.886f, 3.1f, 2.360f}},

@@ -130,8 +130,10 @@ __device__ __forceinline__ void act_grads(int act, const float* dh, float* g, fl
 // A tile's operands.  A k-tile is KB bytes of k (128: 64 bf16, 32 fp32; or 64) of BM
 // rows of A and BN of B, in LDS as it comes from memory, in 16-byte chunks that direct
 // loads put where the fragment reads find them without bank conflicts:
-//  - k contiguous: rows of KB / 16 chunks, chunk c of row r at c ^ chunk_swizzle16(r);
-//    a lane's operand is one 16-byte read;
+//  - k contiguous: rows of 8 chunks, chunk c of row r at c ^ (r & 7); a lane's operand
+//    is one 16-byte read.  LDS serves those of lanes 0-3, 12-15, 20-23 and 24-27 (and
+//    the likes of them) at a time, here from 16 different places in the 256 bytes of
+//    all banks: 4 clocks a read (counted), where c ^ (r & 7) ^ ((r >> 3) & 1) takes 8;
 //  - k strided: rows of k, in units of 16 columns (32 bytes of bf16, 64 of
 //    fp32), unit b of row k at b ^ f(k).  bf16 operands come from
 //    ds_read_b64_tr_b16 (attention.hip has its lane layout): a 16-lane group q
@@ -186,7 +188,7 @@ struct TileLoader {
                 const int c = slot ^ (CU * f(r));
                 voff[i] = c < ROWS / CE ? (uint32_t)r * ldb + 16 * c : TILE_NONE;
             } else {
-                chunk = slot ^ chunk_swizzle16<CPR>(r);     // the same for all: passes are multiples of 16 rows
+                chunk = slot ^ (r & 7);    // the same for all: passes are multiples of 16 rows
                 voff[i] = (uint32_t)row_of(r) * ldb + 16 * chunk;
             }
         }
@@ -234,7 +236,7 @@ struct TileReader {
     uint32_t off;         // this lane's place
     __device__ __forceinline__ void init(int lane) {
         const int r = lane & 15, q = lane >> 4;
-        if constexpr (!STRIDED) off = r * KB + 16 * (q ^ chunk_swizzle16<KB / 16>(r));
+        if constexpr (!STRIDED) off = r * KB + 16 * (q ^ (r & 7));
         else if constexpr (ES == 2) off = (8 * q + (r >> 2)) * RB + 32 * ((r >> 2) + 4 * (q & 1)) + 8 * (r & 3);
         else off = 4 * q * RB + 64 * q + 4 * r;
     }
