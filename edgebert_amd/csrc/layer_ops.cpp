@@ -24,13 +24,13 @@ bool known_dtype(int32_t dtype) { return dtype == EBH_DTYPE_F32 || dtype == EBH_
 bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 uintptr_t element(int32_t dtype) { return dtype == EBH_DTYPE_BF16 ? 2 : 4; }
 
-constexpr int32_t kNormMaxH = 8192, kFfnMaxDim = 65536;
+constexpr int32_t kNormMaxH = 8192, kFfnMaxDim = 65536, kFfnMaxRows = 1 << 30;
 
 int check_ffn(int32_t M, int32_t H, int32_t I, int32_t dtype) {
     if (!known_dtype(dtype)) return fail(EBH_ERR_INVALID_ARG, "unknown dtype %d", dtype);
-    if (M < 0 || H <= 0 || I <= 0 || H % 8 || I % 8 || H > kFfnMaxDim || I > kFfnMaxDim)
-        return fail(EBH_ERR_INVALID_ARG, "bad FFN shape: M %d, H %d, I %d (H and I multiples of 8, at most %d)", M, H, I,
-                    kFfnMaxDim);
+    if (M < 0 || M > kFfnMaxRows || H <= 0 || I <= 0 || H % 8 || I % 8 || H > kFfnMaxDim || I > kFfnMaxDim)
+        return fail(EBH_ERR_INVALID_ARG, "bad FFN shape: M %d (at most %d), H %d, I %d (multiples of 8, at most %d)", M, kFfnMaxRows,
+                    H, I, kFfnMaxDim);
     if (2 * (int64_t)H * I * (int64_t)element(dtype) >= 0xFFFF0000ll)   // 32-bit offsets within the weights
         return fail(EBH_ERR_INVALID_ARG, "FFN weights too large: 2 H I = %lld elements", 2 * (long long)H * I);
     return EBH_OK;

@@ -606,6 +606,77 @@ def test_gradients_against_differences(env):
 
 
 # ---------------------------------------------------------------------------
+# Offsets past 32 bits
+# ---------------------------------------------------------------------------
+def test_rows_past_32_bit_offsets(env):
+    """Rotary positions and layer norm over three rows 4.4 GB apart."""
+    torch, N, L = env
+    H, ld = 256, 2_200_000_000
+    assert ld * 2 > 2 ** 32
+    big = torch.zeros(2 * ld + H, device="cuda", dtype=torch.bfloat16)
+    rows = big.as_strided((3, H), (ld, 1))
+    g = torch.Generator(device="cuda").manual_seed(8)
+    x = torch.randn(3, H, generator=g, device="cuda").to(torch.bfloat16)
+    pos = torch.tensor([5, 77, 300], device="cuda", dtype=torch.int32)
+    cfg = rope_cfg(N, 64)
+
+    def both(src, sld, dst, dld, base):
+        mean, rstd = base.float().mean(1), 1 / base.float().std(1)
+        dg, db = torch.empty(H, device="cuda"), torch.empty(H, device="cuda")
+        size = L.ebh_op_layer_norm_bwd_workspace(3, H)
+        ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+        outs = []
+        for call in (lambda: L.ebh_op_rope(ptr(src), sld, ptr(dst), dld, 1, ptr(pos), None, 3, 4, 64, ctypes.byref(cfg), 0, stream(torch)),
+                     lambda: L.ebh_op_layer_norm_fwd(ptr(src), sld, 1, None, None, 3, H, 1e-5, ptr(dst), dld, None, None, stream(torch)),
+                     lambda: L.ebh_op_layer_norm_bwd(ptr(src), sld, ptr(src), sld, 1, None, ptr(mean), ptr(rstd), ptr(src), sld, 3, H,
+                                                     ptr(dst), dld, ptr(dg), ptr(db), ptr(ws), size, stream(torch))):
+            src.copy_(base)
+            N.check(call())
+            outs.append(dst.clone())
+        return outs + [dg.clone(), db.clone()]
+
+    near_rows = torch.empty(3, H, device="cuda", dtype=torch.bfloat16)
+    want = both(x.clone(), H, near_rows, H, x)
+    got = both(rows, ld, rows, ld, x)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    del big, rows
+    torch.cuda.empty_cache()
+
+
+def test_gated_ffn_activations_past_4_gb(env):
+    """560,000 tokens, g | u and their gradients of 4.6 GB each: the last tokens have
+    the bits of a call of their own, weight gradients are near a sum over parts in 64 bits."""
+    torch, N, L = env
+    M, H, I, tail = 560_000, 64, 2048, 1000
+    assert M * 2 * I * 2 > 2 ** 32
+    c = ffn_case(torch, M, H, I, True, True, 3)
+    y, h, gu = run_ffn(env, c, 0)
+    got = run_ffn_bwd(env, c, 0, h, gu)
+    t = {**c, "M": tail, "x": c["x"][-tail:], "dy": c["dy"][-tail:]}
+    ty, th, tgu = run_ffn(env, t, 0)
+    for a, b in ((y, ty), (h, th), (gu, tgu)):
+        near(torch, a[-tail:], b, 2 ** -7 * b.double().abs() + 1e-3, "the last tokens")
+    g, u = tgu[:, :I].double(), tgu[:, I:].double()
+    a64, d64 = act64(torch, g, 0)
+    dh = t["dy"].double() @ c["wd"].double()
+    dgu = torch.cat([dh * u * d64, dh * a64], 1)
+    wgu = c["wgu"].double()
+    want = dgu @ wgu
+    near(torch, got["dx"][-tail:], want, product_tol(torch, dgu, wgu, 2 ** -7) + 2 ** -8 * want.abs() + 1e-4, "dx of the last tokens")
+    dwd, dbd = torch.zeros(H, I, device="cuda", dtype=torch.float64), torch.zeros(H, device="cuda", dtype=torch.float64)
+    for at in range(0, M, 70_000):
+        dy = c["dy"][at:at + 70_000].double()
+        dwd += dy.T @ h[at:at + 70_000].double()
+        dbd += dy.sum(0)
+    ny, nh = c["dy"].float().norm(dim=0).double(), h.float().norm(dim=0).double()
+    near(torch, got["dwd"], dwd, 4 * (M ** 0.5 + 4) * U * ny[:, None] * nh[None] + 2 ** -8 * dwd.abs(), "dwd")
+    near(torch, got["dbd"][0], dbd, 4 * (M ** 0.5 + 4) * U * M ** 0.5 * ny, "dbd")
+    del c, y, h, gu, got
+    torch.cuda.empty_cache()
+
+
+# ---------------------------------------------------------------------------
 # Together, as a layer and a training step run them
 # ---------------------------------------------------------------------------
 def test_rotary_attention_over_packed_sequences(env):

@@ -34,8 +34,7 @@ def rope_args(**kw):
 
 @pytest.mark.parametrize("kw,words", [
     (dict(cfg=None), "null rope config"), (dict(dtype=2), "unknown dtype"), (dict(dtype=-1), "unknown dtype"),
-    (dict(T=-1), "bad rope shape"), (dict(n=0), "bad rope shape"), (dict(d=0), "bad rope shape"), (dict(d=1025), "bad rope shape"),
-    (dict(n=2 ** 21, d=1024), "bad rope shape"),
+    (dict(T=-1), "bad rope shape"), (dict(n=0), "bad rope shape"), (dict(n=65537), "bad rope shape"), (dict(d=0), "bad rope shape"), (dict(d=1025), "bad rope shape"),
     (dict(rot_dim=31), "rot_dim"), (dict(rot_dim=0), "rot_dim"), (dict(rot_dim=-2), "rot_dim"), (dict(rot_dim=34), "rot_dim"),
     (dict(layout=2), "layout"), (dict(scaling=4), "scaling"), (dict(scaling=-1), "scaling"),
     (dict(base=0.0), "base"), (dict(base=float("nan")), "base"), (dict(base=float("inf")), "base"),
@@ -105,7 +104,7 @@ def ffn_bwd(**kw):
     return list(a.values())
 
 
-SHAPES = [(dict(dtype=2), "unknown dtype"), (dict(M=-1), "shape"), (dict(H=0), "shape"), (dict(I=0), "shape"), (dict(H=60), "shape"),
+SHAPES = [(dict(dtype=2), "unknown dtype"), (dict(M=-1), "shape"), (dict(M=2 ** 30 + 1), "shape"), (dict(H=0), "shape"), (dict(I=0), "shape"), (dict(H=60), "shape"),
           (dict(I=68), "shape"), (dict(H=65544, ldx=65544), "shape"), (dict(I=65544), "shape"), (dict(H=32768, I=32768, ldx=32768), "too large"), (dict(act=3), "activation"),
           (dict(act=-1), "activation")]
 
@@ -152,6 +151,6 @@ def test_workspace_sizes(L):
     # [dg du] of every token is held
     assert L.ebh_op_gated_ffn_bwd_workspace(5000, 768, 2048, 1) >= 5000 * 4096 * 2
     # sizes past 32 bits
-    assert L.ebh_op_gated_ffn_bwd_workspace(2 ** 31 - 1, 768, 2048, 0) >= (2 ** 31 - 1) * 4096 * 4
+    assert L.ebh_op_gated_ffn_bwd_workspace(2 ** 30, 768, 2048, 0) >= 2 ** 30 * 4096 * 4
     # a bound on what a caller has to keep for norms, however many rows
     assert max(L.ebh_op_layer_norm_bwd_workspace(r, 768) for r in (1, 1000, 2 ** 31 - 1)) <= 64 << 20
