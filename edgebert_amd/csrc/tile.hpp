@@ -152,7 +152,7 @@ constexpr uint32_t TILE_NONE = 0x80000000u;   // past every output's rows in a t
 template <bool STRIDED, int ROWS>
 constexpr int tile_pitch() { return STRIDED && ROWS == 192 ? 256 : ROWS; }
 
-template <class T, bool STRIDED, int ROWS, int KB, int NT, bool PLAIN>
+template <class T, bool STRIDED, int ROWS, int KB, int NT>
 struct TileLoader {
     static constexpr int ES = sizeof(T), KT = KB / ES, CE = 16 / ES, PITCH = tile_pitch<STRIDED, ROWS>();
     static constexpr int L = PITCH * (KB / 16) / NT;   // loads per thread and k-tile
@@ -166,30 +166,35 @@ struct TileLoader {
     }
 
     uint32_t ldb;         // bytes between rows
-    // A pass's chunks lie a fixed number of rows behind the one before's, except where
-    // the swizzle (fp32, strided) or the panel's rows (the gate's) go another way
-    static constexpr bool EVEN = PLAIN && PITCH == ROWS && (!STRIDED || (ES == 2 && RPL % 16 == 0));
-    uint32_t voff[L];     // this thread's chunks, from the k-tile's start
+    // A pass's chunks lie RPL rows behind the one's before; strided, the swizzle has them
+    // in another place where RPL is not its period (16 rows of k in bf16, fp32 too).
+    static constexpr int BASES = !STRIDED || RPL % 16 == 0 ? 1 : 16 / RPL;
+    static_assert(BASES <= L, "passes");
+    uint32_t voff[BASES]; // this thread's chunks, from the k-tile's start
+    uint32_t other;       // the gate's tile: bytes from the gate's rows to the other projection's
     int chunk;            // k contiguous: the chunk's place in k
     uint64_t base;        // of the next k-tile to load
     uint32_t size;        // k contiguous: bytes from there to the panel's end
     int left;             // k from there to the end
     uint32_t last;        // k strided: bytes of a row from the panel's first column to the operand's last
 
-    // row_of(r): the row of the operand's panel that goes to row r in LDS.
-    template <class F>
-    __device__ __forceinline__ void init(int64_t ld, int tid, F&& row_of) {
+    // HALF > 0: every other HALF rows in LDS are the other projection's, `second` rows on.
+    template <int HALF = 0>
+    __device__ __forceinline__ void init(int64_t ld, int tid, int second = 0) {
+        static_assert(HALF == 0 || (!STRIDED && (RPL == HALF || RPL % (2 * HALF) == 0)), "whole passes");
         ldb = (uint32_t)(ld * ES);
+        other = (uint32_t)second * ldb;
         chunk = 0;
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
+        for (int i = 0; i < BASES; ++i) {
             const int r = tid / CPR + i * RPL, slot = tid % CPR;
             if constexpr (STRIDED) {
                 const int c = slot ^ (CU * f(r));
                 voff[i] = c < ROWS / CE ? (uint32_t)r * ldb + 16 * c : TILE_NONE;
             } else {
-                chunk = slot ^ (r & 7);    // the same for all: passes are multiples of 16 rows
-                voff[i] = (uint32_t)row_of(r) * ldb + 16 * chunk;
+                chunk = slot ^ (r & 7);                   // the same for all: passes are multiples of 16 rows
+                const int row = HALF > 0 ? r / (2 * HALF) * HALF + r % HALF : r;
+                voff[i] = (uint32_t)row * ldb + 16 * chunk + (HALF > 0 && r % (2 * HALF) >= HALF ? other : 0u);
             }
         }
     }
@@ -204,20 +209,38 @@ struct TileLoader {
             size = left > 0 ? (uint32_t)((rows - r0 - 1) * ld + left) * ES : 0u;   // less than 2^32: layer_ops.cpp
         }
     }
-    // The next k-tile's loads, one at a time, into LDS at `lds` (this wave's part of the stage).
-    __device__ __forceinline__ void load(int i, uint32_t lds) const {
+    // The next k-tile's loads, into LDS at `lds` (this wave's part of the stage).
+    template <int HALF = 0>
+    __device__ __forceinline__ void load(uint32_t lds) const {
         uint32_t bytes;
         if constexpr (STRIDED) bytes = left > 0 ? (uint32_t)(min(left, KT) - 1) * ldb + last : 0u;
         else bytes = left > 0 ? size : 0u;
         const g16_v4i rsrc = {(int)(uint32_t)base, (int)((uint32_t)(base >> 32) & 0xffffu), (int)bytes, G16_RSRC_WORD3};
-        uint32_t v = EVEN ? voff[0] + i * RPL * ldb : voff[i];
         // k ends inside this k-tile: what lies behind it in a row is not zeros
-        if (!STRIDED && left < KT) v = chunk * CE >= left ? TILE_OUT : v;
-        asm volatile(
-            "s_mov_b32 m0, %2\n\t"
-            "s_nop 0\n\t"
-            "buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(v), "s"(rsrc), "s"(lds + i * NT * 16)
-            : "memory", "m0");
+        const uint32_t out = !STRIDED && left < KT && chunk * CE >= left ? TILE_OUT : 0u;
+        uint32_t v[BASES], row = ldb;
+        asm volatile("" : "+s"(row));              // multiples are formed here, one after the other
+#pragma unroll
+        for (int i = 0; i < BASES; ++i) v[i] = voff[i];
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            uint32_t at = v[i % BASES];
+            if constexpr (HALF > 0 && RPL < 2 * HALF) {
+                // RPL rows on in LDS: the other projection's, or the gate's next ones
+                static_assert(RPL == HALF, "a pass is one projection's");
+                if (i & 1) {
+                    at += other;
+                    v[0] += HALF * row;
+                }
+            } else {
+                v[i % BASES] += (HALF > 0 ? RPL / 2 : BASES * RPL) * row;
+            }
+            asm volatile(
+                "s_add_u32 m0, %2, %3\n\t"
+                "s_nop 0\n\t"
+                "buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(STRIDED ? at : at | out), "s"(rsrc), "s"(lds), "n"(i * NT * 16)
+                : "memory", "m0", "scc");
+        }
     }
     __device__ __forceinline__ void advance() {
         left -= KT;
@@ -326,6 +349,7 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
     static_assert(FM * 16 == WM && FN * 16 == WN && FN % (USE == USE_GATE ? 4 : 2) == 0, "pairs of blocks");
     constexpr int SB = FM >= 8 ? 2 : 1, STEPS = FM / SB;
     static_assert(STEPS % 2 == 0, "steps alternate between two A sets");
+    static_assert(NT == 256 || (NT == 512 && NS == 2), "turns of loading go with the two stages");
     constexpr int OS = USE == USE_PARTIAL ? 4 : ES;        // bytes of a stored element
     constexpr int FC = USE == USE_GATE ? FN / 2 : FN;      // blocks of a wave's columns of C
     constexpr int BNC = USE == USE_GATE ? BN / 2 : BN;     // columns of C in a tile
@@ -333,7 +357,7 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
     constexpr int NLD = (ST_A + ST_B) / 16 / NT;                // loads per thread and k-tile
     constexpr int NSTO = FM * FC * OS / 4;                 // stores per thread and tile, at least
 
-    const int ntn = (p.N + BNC - 1) / BNC, ntiles = ((p.M + BM - 1) / BM) * ntn, nwork = ntiles * p.splits, nk = p.kt_split;
+    const int ntn = (p.N + BNC - 1) / BNC, ntiles = ((p.M + BM - 1) / BM) * ntn, nwork = ntiles * (USE == USE_PARTIAL ? p.splits : 1), nk = p.kt_split;
     // Workgroup b runs on XCD b % 8; each XCD's workgroups take consecutive items,
     // which share operand panels in that XCD's L2.
     const int grid = gridDim.x;
@@ -348,53 +372,57 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
     }
     const int my_tiles = u0 < uend ? (uend - u0 + ustep - 1) / ustep : 0;
     if (my_tiles == 0) return;   // uniform over the workgroup
-    // One workgroup a CU: neighbours in an XCD start 2,048 clocks apart, in four
-    // phases, or the whole chip would load, multiply and store in step (32,768
-    // rows, 768 -> 2 x 2,048: 250 -> 188 us; the slopes of it 193 -> 183 us)
-    if constexpr (NT == 512)
-        for (int w = (blockIdx.x >> 3) & 3; w > 0; --w) __builtin_amdgcn_s_sleep(32);
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WAVES_N, wn = wave % WAVES_N;
-    const uint32_t lds0 = (uint32_t)(uintptr_t)smem + (uint32_t)wave * 1024;
 
-    TileLoader<T, AKS, BM, KB, NT, true> la;
-    TileLoader<T, BKS, BN, KB, NT, USE != USE_GATE> lb;
-    la.init(p.lda, tid, [](int r) { return r; });
+    // Eight waves load by turns, one k-tile the first four and one the others (mfma_step).
+    constexpr int LT = NT == 512 ? 256 : NT, HALF = USE == USE_GATE ? WN / 2 : 0;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)smem + (uint32_t)(wave % (LT / 64)) * 1024;
+    TileLoader<T, AKS, BM, KB, LT> la;
+    TileLoader<T, BKS, BN, KB, LT> lb;
+    la.init(p.lda, tid % LT);
     // USE_GATE: half of each wave's columns are the gate's, the others the same ones of the other projection
-    lb.init(p.ldb, tid, [&](int r) { return USE == USE_GATE ? r / WN * (WN / 2) + r % (WN / 2) + (r % WN < WN / 2 ? 0 : p.N) : r; });
+    lb.template init<HALF>(p.ldb, tid % LT, p.N);
     int lt = 0, lkt = 0, li = 0;   // the stream's next k-tile: its item, its place in it, its number
+    int ls = 0, its = 0;           // of three stages and more: its one, and that of the one being multiplied
     auto item = [&](int t, int& m0, int& n0, int& split) __attribute__((always_inline)) {
+        int across = ntn, all = ntiles;
+        asm volatile("" : "+s"(across), "+s"(all));   // their reciprocals are formed here, not held across the k-loop
         const int u = u0 + t * ustep;
-        split = u / ntiles;
-        const int tile = u - split * ntiles, mt = tile / ntn;
+        split = USE == USE_PARTIAL ? u / all : 0;
+        const int tile = u - split * all, mt = tile / across;
         m0 = mt * BM;
-        n0 = (tile - mt * ntn) * BNC;
+        n0 = (tile - mt * across) * BNC;
     };
+    typedef const __attribute__((address_space(4))) TileArgs* Args;
     auto cursors = [&](int t) __attribute__((always_inline)) {
         int m0, n0, split;
         item(t, m0, n0, split);
         const int64_t k0 = (int64_t)split * nk * KT;
-        la.at(p.A, p.lda, m0, AKS ? p.M : min(p.M, m0 + BM), k0, p.K);
-        lb.at(p.B, p.ldb, n0, USE == USE_GATE ? 2 * (int64_t)p.N : (BKS ? p.N : min(p.N, n0 + BN)), k0, p.K);
+        // The arguments (the kernel's only one, at its arguments' start) come from memory
+        // anew, here and in finish(): held across the k-loop they would spill scalar
+        // registers.
+        Args ep = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(ep));
+        const int M = ep->M, N = ep->N, K = ep->K, lda = ep->lda, ldb = ep->ldb;
+        la.at(ep->A, lda, m0, AKS ? M : min(M, m0 + BM), k0, K);
+        lb.at(ep->B, ldb, n0, USE == USE_GATE ? 2 * (int64_t)N : (BKS ? N : min(N, n0 + BN)), k0, K);
     };
-    // The next k-tile's loads n .. n + count - 1 of this thread, into the stage of its
-    // number, even or odd (k-tiles come in pairs) or by the count.
-    constexpr int LA = decltype(la)::L, LOADS = LA + decltype(lb)::L;
-    auto loads = [&](int n, int count, int par) __attribute__((always_inline)) {
-        if (lt >= my_tiles) return;
-        const uint32_t st = NS == 2 ? par : li % NS;
-#pragma unroll
-        for (int i = n; i < n + count && i < LOADS; ++i) {
-            if (i < LA) la.load(i, lds0 + st * ST_A);
-            else lb.load(i - LA, lds0 + B_OFF + st * ST_B);
-        }
+    // The next k-tile's loads of A and of B, into the stage of its number, even or odd
+    // (k-tiles come in pairs), or the next of three and more.
+    auto load_a = [&](int par) __attribute__((always_inline)) {
+        if (lt < my_tiles) la.load(lds0 + (uint32_t)(NS == 2 ? par : ls) * ST_A);
+    };
+    auto load_b = [&](int par) __attribute__((always_inline)) {
+        if (lt < my_tiles) lb.template load<HALF>(lds0 + B_OFF + (uint32_t)(NS == 2 ? par : ls) * ST_B);
     };
     auto next = [&]() __attribute__((always_inline)) {
         if (lt >= my_tiles) return;
         la.advance();
         lb.advance();
         ++li;
+        ls = ls + 1 == NS ? 0 : ls + 1;
         if (++lkt == nk) {
             lkt = 0;
             if (++lt < my_tiles) cursors(lt);
@@ -424,11 +452,13 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
         }
         lds_barrier();
     };
-    // One step's MFMAs.  A load holds up its wave until the CU's address unit has
-    // taken it, 16 clocks for each of the workgroup's waves: they go out one by one
-    // between the MFMAs, in the first half of a k-tile's slots (one after every
-    // FN); two workgroups a CU do with A's and B's in one go each.
-    constexpr int SLOTS = SB * SL, PER = NT == 256 ? LA : (2 * LOADS + STEPS * SLOTS - 1) / (STEPS * SLOTS);
+    // One step's MFMAs.  A load holds up its wave until the CU's address unit takes
+    // it, 16 clocks for each: half of a k-tile's MFMA time for all of its loads.  So
+    // of the two waves of a SIMD one loads, for both, while the other has the matrix
+    // core (32,768 rows, 768 x 2,048: 326 -> 321 us forward, 696 -> 685 back, over
+    // every wave's own loads one by one between its MFMAs); two workgroups of four
+    // waves a CU do so of themselves, with A's and B's loads in one go each, after the
+    // first FN MFMAs (`slot`) and the second.
     auto mfma_step = [&](int s, int as, int bs, int slot, int par) __attribute__((always_inline)) {
 #pragma unroll
         for (int sl = 0; sl < SL; ++sl)
@@ -445,9 +475,9 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
                         else
                             d = __builtin_amdgcn_mfma_f32_16x16x4f32(bf[bs][j][sl][e], af[as][i][sl][e], d, 0, 0, 0);
                     }
-                if (slot >= 0 && slot * PER < LOADS) {
+                if (NT == 256 && (slot == 0 || slot == 1)) {
                     __builtin_amdgcn_sched_barrier(0);
-                    loads(slot * PER, PER, par);
+                    slot ? load_b(par) : load_a(par);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 ++slot;
@@ -455,7 +485,7 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
     };
     auto run_ktile = [&](auto set, bool first) __attribute__((always_inline)) {
         constexpr int P = decltype(set)::value;
-        const int st = NS == 2 ? P : it % NS;
+        const int st = NS == 2 ? P : its;
         const char *sa = smem + st * ST_A, *sb = smem + B_OFF + st * ST_B;
         auto rd_a = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
@@ -472,30 +502,35 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
             for (int sl = 0; sl < SL; ++sl) bf[P][j][sl] = rb.read(sb, wn * FN + j, sl);
         __builtin_amdgcn_sched_barrier(0);            // reads stay ahead of the MFMAs that hide them
         constexpr int par = NS == 2 ? P ^ 1 : 0;
+        if (NT == 512 && (wave >> 2) == P) {
+            load_a(par);
+            load_b(par);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         if (!first) mfma_step(STEPS - 1, 1, P ^ 1, 0, par);   // the previous k-tile's last step
-        else loads(0, SLOTS * PER, par);
+        else if (NT == 256) {
+            load_a(par);
+            load_b(par);
+        }
 #pragma unroll
         for (int s = 0; s + 1 < STEPS; ++s) {
             rd_a(s + 1);
             __builtin_amdgcn_sched_barrier(0);
-            mfma_step(s, s & 1, P, (s + 1) * SLOTS, par);
+            mfma_step(s, s & 1, P, 2, par);
             __builtin_amdgcn_sched_barrier(0);
         }
         next();
         ++it;
+        its = its + 1 == NS ? 0 : its + 1;
     };
 
     auto finish = [&](int t) __attribute__((always_inline)) {
         int m0, n0, split;
         item(t, m0, n0, split);
-        // What only this part reads of the arguments (the kernel's only one, at its
-        // arguments' start) comes from memory now: held across the k-loop it would
-        // spill scalar registers.
-        typedef const __attribute__((address_space(4))) TileArgs* Args;
         Args ep = (Args)__builtin_amdgcn_kernarg_segment_ptr();
         asm volatile("" : "+s"(ep));
         const float* const biases = ep->bias;
-        const int I = ep->I, act = ep->act;
+        const int M = ep->M, N = ep->N, I = ep->I, act = ep->act;
         const int wrow = m0 + wm * WM;
         int el = lane;
         asm volatile("" : "+v"(el));   // formed here, not held across the k-loop
@@ -507,21 +542,21 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
         auto places = [&](int jp, int bytes, uint32_t* o) __attribute__((always_inline)) {
             const int w = cbase + 32 * jp + 16 * (q & 1) + 8 * (q >> 1);
             if constexpr (OS == 2) {
-                o[0] = w < p.N ? (uint32_t)(r * bytes + w * 2) : TILE_NONE;
+                o[0] = w < N ? (uint32_t)(r * bytes + w * 2) : TILE_NONE;
             } else {
 #pragma unroll
-                for (int b = 0; b < 2; ++b) o[b] = col(2 * jp + b) < p.N ? (uint32_t)(r * bytes + col(2 * jp + b) * 4) : TILE_NONE;
+                for (int b = 0; b < 2; ++b) o[b] = col(2 * jp + b) < N ? (uint32_t)(r * bytes + col(2 * jp + b) * 4) : TILE_NONE;
             }
         };
         // The wave's rows of a matrix; a lane's places in them are less than 2^31 from
         // the first, and TILE_NONE is past them
         auto rows = [&](const void* base, int bytes) __attribute__((always_inline)) {
-            const int left = __builtin_amdgcn_readfirstlane(min(p.M - wrow, WM));
+            const int left = __builtin_amdgcn_readfirstlane(min(M - wrow, WM));
             return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(base) + (int64_t)wrow * bytes),
                                                      (short)0, (left > 0 ? left : 0) * bytes, G16_RSRC_WORD3);
         };
         auto bias = [&](int j, const float* from, float* v) __attribute__((always_inline)) {
-            const bool in = from && col(j) < p.N;
+            const bool in = from && col(j) < N;
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = in ? from[col(j) + e] : 0.0f;
         };
@@ -529,7 +564,7 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
         if constexpr (USE == USE_STORE || USE == USE_PARTIAL) {
             int bytes = ep->ldc * OS;
             asm volatile("" : "+s"(bytes));   // its multiples are formed here, not held
-            const auto d = rows(static_cast<char*>(ep->C) + (USE == USE_PARTIAL ? (int64_t)split * p.M * bytes : 0), bytes);
+            const auto d = rows(static_cast<char*>(ep->C) + (USE == USE_PARTIAL ? (int64_t)split * M * bytes : 0), bytes);
             float bv[FN][4];
             uint32_t o[FN / 2][2];
 #pragma unroll
@@ -589,8 +624,8 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
                     }
             } else {
                 const auto src = rows(gu, row_gu), dst = rows(ep->dgu, row_gu);
-                constexpr int N = FM * FN / 2, AHEAD = N < 4 ? N : 4;   // pairs of blocks, and how many's g and u are on their way
-                float* const colsum = ep->colsum;
+                constexpr int PAIRS = FM * FN / 2, AHEAD = 2;   // pairs of blocks, and how many's g and u are on their way
+                const bool sums = ep->colsum != nullptr;
                 float cg[FN][4] = {}, cu[FN][4] = {};
                 RawBlocks<ES> raw[AHEAD][2];
                 // pair k, `rows16` rows of blocks on from where og has come to
@@ -601,18 +636,18 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
 #pragma unroll
                 for (int k = 0; k < AHEAD; ++k) load(k, k / (FN / 2));
 #pragma unroll
-                for (int k = 0; k < N; ++k) {
+                for (int k = 0; k < PAIRS; ++k) {
                     const int i = k / (FN / 2), jp = k % (FN / 2);
                     float g[2][4], u[2][4], dh[2][4];
                     raw[k % AHEAD][0].values(g[0], g[1]);
                     raw[k % AHEAD][1].values(u[0], u[1]);
-                    if (k + AHEAD < N) load(k + AHEAD, (k + AHEAD) / (FN / 2) - i);
+                    if (k + AHEAD < PAIRS) load(k + AHEAD, (k + AHEAD) / (FN / 2) - i);
 #pragma unroll
                     for (int b = 0; b < 2; ++b)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) dh[b][e] = acc[i][2 * jp + b][e];
                     act_grads<8>(act, dh[0], g[0], u[0]);
-                    if (colsum) {
+                    if (sums) {
 #pragma unroll
                         for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -627,7 +662,9 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
                     og[jp][1] += 16 * row_gu;
                     __builtin_amdgcn_sched_barrier(0);   // keeps the loads so far ahead, not all of them
                 }
-                if (colsum) {
+                if (sums) {
+                    asm volatile("" : "+s"(ep));
+                    float* const colsum = ep->colsum;
                     // rows past the last are zeros: dh is, of operands that are
 #pragma unroll
                     for (int j = 0; j < FN; ++j) {
@@ -638,7 +675,7 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
                                 cg[j][e] += __shfl_xor(cg[j][e], o);
                                 cu[j][e] += __shfl_xor(cu[j][e], o);
                             }
-                        if (r == 0 && col(j) < p.N) {
+                        if (r == 0 && col(j) < N) {
                             float* at = colsum + (int64_t)(m0 / BM * WAVES_M + wm) * 2 * I + col(j);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
@@ -655,7 +692,10 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
     cursors(0);
 #pragma unroll
     for (int d = 0; d < NS - 1; ++d) {
-        loads(0, LOADS, d);
+        if (NT == 256 || wave < 4) {
+            load_a(d);
+            load_b(d);
+        }
         next();
     }
     typedef std::integral_constant<int, 0> set0;
@@ -669,13 +709,14 @@ __device__ __forceinline__ void tile_body(const TileArgs& p, char* const smem) {
         run_ktile(set0{}, true);
         enter(NS > 2 && t > 0);
         run_ktile(set1{}, false);
+#pragma unroll 1
         for (int kt = 2; kt < nk; kt += 2) {
             enter(false);
             run_ktile(set0{}, false);
             enter(false);
             run_ktile(set1{}, false);
         }
-        mfma_step(STEPS - 1, 1, 1, -SLOTS, 0);
+        mfma_step(STEPS - 1, 1, 1, 2, 0);
         finish(t);
     }
 }
