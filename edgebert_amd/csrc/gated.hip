@@ -14,12 +14,13 @@ namespace ebh {
 struct TileShape {
     int bm, bn, waves_m, waves_n, ns;
 };
-constexpr int TILES = 4, TILE_KB = 128;
+constexpr int TILES = 5, TILE_KB = 128;
 constexpr TileShape kTiles[TILES] = {
     {256, 256, 2, 4, 2},   // 8 waves, one workgroup a CU
     {256, 192, 4, 2, 2},
     {128, 128, 2, 2, 2},   // 4 waves, two a CU
     {64, 128, 2, 2, 3},
+    {64, 64, 2, 2, 3},     // fp32, where few tokens leave CUs idle: 1,061 of 384 x 1,000 back, 108 -> 95 us
 };
 constexpr int tile_threads(int t) { return 64 * kTiles[t].waves_m * kTiles[t].waves_n; }
 
@@ -88,8 +89,9 @@ static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 //   launch + full rounds * (k/64 * full + epi) + a last one of one workgroup
 //   (k/64 * one + epi / 2).
 // Constants fitted to a sweep on MI355X of the five products at 70 .. 32,768
-// tokens of H 384 .. 1,024, I 1,000 .. 4,096 and 1 .. 24 splits (rms error 4-14%;
-// the choice takes 1.01-1.02 times the best's time on average, at worst 1.23).
+// tokens of H 384 .. 1,024, I 1,000 .. 4,096 and 1 .. 24 splits (rms error 4-14%,
+// fp32 1-4%; the choice takes 1.01-1.02 times the best's time on average, at worst
+// 1.23).
 // What they say: the largest tile runs its k fastest but needs whole rounds of
 // 256; few tiles are split over k, as long as writing and reading the partial
 // sums (6 TB/s, and a launch) costs less than the idle CUs.
@@ -102,16 +104,17 @@ static const TileTime kTimes[2][4][TILES] = {   // bf16, fp32; by Use
      {{1.2f, 1.363f, 11.3f, 0}, {2.8f, 1.165f, 7.8f, 0}, {2.5f, 0.883f, 5.0f, 0.644f}, {3.7f, 0.602f, 2.2f, 0.403f}},
      {{2.1f, 1.414f, 5.6f, 0}, {}, {3.5f, 1.082f, 0.4f, 0.617f}, {2.6f, 0.893f, 0.0f, 0.610f}},
      {{0.0f, 1.282f, 20.5f, 0}, {}, {0.0f, 0.732f, 14.4f, 0.505f}, {2.1f, 0.743f, 4.7f, 0.511f}}},
-    {{{}, {}, {5.5f, 7.39f, 4.0f, 3.963f}, {0.0f, 4.119f, 5.4f, 2.489f}},
-     {{}, {}, {3.9f, 7.389f, 3.8f, 3.994f}, {3.8f, 4.013f, 1.8f, 2.374f}},
-     {{}, {}, {0.0f, 6.766f, 10.4f, 3.953f}, {3.2f, 3.886f, 3.1f, 2.360f}},
-     {{}, {}, {0.2f, 6.804f, 23.2f, 3.665f}, {0.0f, 3.202f, 13.9f, 2.352f}}},
+    {{{}, {}, {3.9f, 7.389f, 3.8f, 3.994f}, {0.0f, 4.211f, 2.7f, 2.493f}, {0.9f, 2.124f, 4.0f, 1.393f}},
+     {{}, {}, {3.6f, 7.474f, 4.4f, 4.015f}, {3.3f, 4.096f, 2.2f, 2.393f}, {3.1f, 2.112f, 1.5f, 1.360f}},
+     {{}, {}, {4.2f, 7.379f, 1.6f, 3.878f}, {3.8f, 4.063f, 1.0f, 2.269f}, {}},
+     {{}, {}, {1.0f, 7.367f, 16.2f, 4.052f}, {2.7f, 3.850f, 7.5f, 2.404f}, {3.3f, 2.244f, 2.3f, 1.416f}}},
 };
 
-// Whether a product can have a tile: fp32 tiles are the small ones; a strided A has
-// at least 128 columns; the gate's waves have pairs of blocks of each projection.
+// Whether a product can have a tile: fp32 tiles are the small ones, and bf16's strided
+// operands have at least 128 columns; the gate's waves have pairs of blocks of each
+// projection.
 constexpr bool has_tile(int t, bool bf16, bool a_strided, int use) {
-    return (bf16 || t >= 2) && !(a_strided && t == 3) && !(t == 1 && (use == USE_GATE || use == USE_SLOPES));
+    return (bf16 ? t < 4 : t >= 2) && !(bf16 && a_strided && t == 3) && !(t == 1 && (use == USE_GATE || use == USE_SLOPES)) && !(t == 4 && use == USE_GATE);
 }
 
 struct Plan {
@@ -423,15 +426,19 @@ static BwdSpace bwd_space(int M, int H, int I, bool bf16) {
 int64_t gated_bwd_ws_bytes(int M, int H, int I, bool bf16) { return bwd_space(M, H, I, bf16).bytes; }
 
 template <class T>
-static void gated_bwd(const GatedArgs& g, hipStream_t s) {
+static hipError_t gated_bwd(const GatedArgs& g, hipStream_t s) {
     const int64_t I2 = 2 * (int64_t)g.I;
     if (g.M == 0) {   // sums over no rows
         const int64_t words = sizeof(T) * g.H * (int64_t)g.I / 4;
-        if (g.dWgu) launch_zero_words(g.dWgu, 2 * words, s);
-        if (g.dWd) launch_zero_words(g.dWd, words, s);
-        if (g.dbgu) launch_zero_words(g.dbgu, I2, s);
-        if (g.dbd) launch_zero_words(g.dbd, g.H, s);
-        return;
+        hipError_t e = hipSuccess;
+        auto zero = [&](void* p, int64_t n) {
+            if (p && e == hipSuccess) e = launch_zero_words(p, n, s);
+        };
+        zero(g.dWgu, 2 * words);
+        zero(g.dWd, words);
+        zero(g.dbgu, I2);
+        zero(g.dbd, g.H);
+        return e;
     }
     const BwdSpace w = bwd_space(g.M, g.H, g.I, sizeof(T) == 2);
     char* const ws = static_cast<char*>(g.ws);
@@ -494,6 +501,7 @@ static void gated_bwd(const GatedArgs& g, hipStream_t s) {
         a.N = g.I;
         stored_product<T, true, true>(a, w.wd, partial, s);
     }
+    return hipGetLastError();
 }
 
 hipError_t launch_gated(const GatedArgs& a, bool bf16, hipStream_t s) {
@@ -503,9 +511,7 @@ hipError_t launch_gated(const GatedArgs& a, bool bf16, hipStream_t s) {
 }
 
 hipError_t launch_gated_bwd(const GatedArgs& a, bool bf16, hipStream_t s) {
-    if (bf16) gated_bwd<uint16_t>(a, s);
-    else gated_bwd<float>(a, s);
-    return hipGetLastError();
+    return bf16 ? gated_bwd<uint16_t>(a, s) : gated_bwd<float>(a, s);
 }
 
 }  // namespace ebh

@@ -7,6 +7,8 @@
 #include "gemm16.hpp"
 #include "layer.hpp"
 
+#pragma clang diagnostic ignored "-Winline-asm"   // m0 among the clobbers, a reserved register
+
 namespace ebh {
 
 // What is done with a tile.
