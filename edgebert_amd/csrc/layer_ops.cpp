@@ -25,6 +25,7 @@ bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 
 uintptr_t element(int32_t dtype) { return dtype == EBH_DTYPE_BF16 ? 2 : 4; }
 
 constexpr int32_t kNormMaxH = 8192, kFfnMaxDim = 65536, kFfnMaxRows = 1 << 30;
+constexpr int32_t kRopeMaxT = 1 << 26;   // 2^23 workgroups of 256 lanes: a grid has less than 2^32
 
 int check_ffn(int32_t M, int32_t H, int32_t I, int32_t dtype) {
     if (!known_dtype(dtype)) return fail(EBH_ERR_INVALID_ARG, "unknown dtype %d", dtype);
@@ -59,8 +60,8 @@ int ebh_op_rope(const void* x, int64_t ldx, void* y, int64_t ldy, int32_t dtype,
                 int32_t transpose, void* stream) {
     if (!cfg) return fail(EBH_ERR_INVALID_ARG, "null rope config");
     if (!known_dtype(dtype)) return fail(EBH_ERR_INVALID_ARG, "unknown dtype %d", dtype);
-    if (T < 0 || n_heads <= 0 || n_heads > 65536 || head_dim <= 0 || head_dim > 1024)
-        return fail(EBH_ERR_INVALID_ARG, "bad rope shape: T %d, %d heads of %d", T, n_heads, head_dim);
+    if (T < 0 || T > kRopeMaxT || n_heads <= 0 || n_heads > 65536 || head_dim <= 0 || head_dim > 1024)
+        return fail(EBH_ERR_INVALID_ARG, "bad rope shape: T %d (at most %d), %d heads of %d", T, kRopeMaxT, n_heads, head_dim);
     const ebh_rope& c = *cfg;
     if (c.rot_dim < 2 || c.rot_dim % 2 || c.rot_dim > head_dim)
         return fail(EBH_ERR_INVALID_ARG, "rot_dim %d: even, 2 .. head_dim %d", c.rot_dim, head_dim);

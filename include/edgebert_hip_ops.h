@@ -257,8 +257,8 @@ typedef struct ebh_rope {
  * k of a qkv row.  y may be x (ldy = ldx).  n_tokens (device, nullable): only the
  * first *n_tokens of the T rows are turned, the others not read nor written.
  * transpose != 0: the transposed map, angle -pos * f_i, which takes a
- * gradient of y to one of x.  Angles are formed in 64 bits.  n_heads <= 65536,
- * head_dim <= 1024, pointers aligned to their elements. */
+ * gradient of y to one of x.  Angles are formed in 64 bits.  T <= 2^26,
+ * n_heads <= 65536, head_dim <= 1024, pointers aligned to their elements. */
 EBH_API int ebh_op_rope(const void* x, int64_t ldx, void* y, int64_t ldy, int32_t dtype, const int32_t* pos,
                 const int32_t* n_tokens, int32_t T, int32_t n_heads, int32_t head_dim, const ebh_rope* cfg,
                 int32_t transpose, void* stream);
@@ -289,11 +289,13 @@ EBH_API int ebh_op_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, i
  * Y = h.Wd^T + bd.  X [M, H] (ldx) and Y [M, H] (ldy); Wgu [2 I, H] holds the
  * gate's I rows, then the other projection's; Wd [H, I]; biases (nullable) bgu
  * [2 I], bd [H].  h [M, I] is written, and read by the second product (bf16:
- * of at most 64 tokens Y is formed of h before its rounding); gu [M, 2 I] (nullable) keeps g | u for the backward pass.  Weights, h and gu are
+ * of at most 64 tokens Y is formed of h before its rounding); gu [M, 2 I]
+ * (nullable) keeps g | u for the backward pass.  Weights, h and gu are
  * contiguous.  act: EBH_ACT_SILU g / (1 + e^-g), EBH_ACT_GELU_TANH (as
  * EBH_EPI_BIAS_GELU) or EBH_ACT_GELU_ERF g/2 (1 + erf(g / sqrt 2)).  M is at most
  * 2^30, H, I and the strides are multiples of 8, H and I at most 65536, 2 H I
- * elements less than 2^32 - 2^16 bytes, strides at most 2,796,202; operands 16-byte aligned.  `workspace` (16-byte aligned, NULL where 0) has
+ * elements less than 2^32 - 2^16 bytes, strides at most 2,796,202; operands are
+ * 16-byte aligned.  `workspace` (16-byte aligned, NULL where 0) has
  * ebh_op_gated_ffn_workspace(M, H, I, dtype) bytes. */
 #define EBH_ACT_SILU 0
 #define EBH_ACT_GELU_TANH 1

@@ -154,3 +154,8 @@ def test_workspace_sizes(L):
     assert L.ebh_op_gated_ffn_bwd_workspace(2 ** 30, 768, 2048, 0) >= 2 ** 30 * 4096 * 4
     # a bound on what a caller has to keep for norms, however many rows
     assert max(L.ebh_op_layer_norm_bwd_workspace(r, 768) for r in (1, 1000, 2 ** 31 - 1)) <= 64 << 20
+
+
+def test_rope_tokens_are_bounded(L):
+    """A grid has less than 2^32 lanes."""
+    refused(L.ebh_op_rope(*rope_args(T=(1 << 26) + 1)), "bad rope shape")
