@@ -800,3 +800,20 @@ def test_steps_on_two_streams_at_once(env):
     for a, b in zip(alone, both):
         for k in RESULTS:
             assert torch.equal(a[k], b[k]), k
+
+
+@pytest.mark.parametrize("M", [1, 20, 64, 65, 300])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_gated_ffn_infinite_products_stay_infinite(env, bf16, M):
+    """g u past the type's largest value is infinite, and so is Y = h.Wd^T of
+    weights above 0, at every size; the other tokens are as without it."""
+    torch, N, L = env
+    c = ffn_case(torch, M, 64, 96, bf16, False, 5)
+    c["wgu"].abs_()
+    c["wd"].abs_().add_(0.25)
+    plain, _, _ = run_ffn(env, c, 0)
+    c["x"][M - 1] = 1e30
+    y, h, _ = run_ffn(env, c, 0)
+    assert bool((h[M - 1] == float("inf")).all()) and bool((y[M - 1] == float("inf")).all())
+    assert torch.equal(y[: M - 1], plain[: M - 1]) and bool(torch.isfinite(plain).all())
+
