@@ -129,7 +129,7 @@ __device__ __forceinline__ void act_grads(int act, const float* dh, float* g, fl
 }
 
 // ---------------------------------------------------------------------------
-// A tile's operands.  A k-tile is KB bytes of k (128: 64 bf16, 32 fp32; or 64) of BM
+// A tile's operands.  A k-tile is KB = 128 bytes of k (64 bf16, 32 fp32) of BM
 // rows of A and BN of B, in LDS as it comes from memory, in 16-byte chunks that direct
 // loads put where the fragment reads find them without bank conflicts:
 //  - k contiguous: rows of 8 chunks, chunk c of row r at c ^ (r & 7); a lane's operand

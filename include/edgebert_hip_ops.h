@@ -295,8 +295,9 @@ EBH_API int ebh_op_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, i
  * EBH_EPI_BIAS_GELU) or EBH_ACT_GELU_ERF g/2 (1 + erf(g / sqrt 2)).  M is at most
  * 2^30, H, I and the strides are multiples of 8, H and I at most 65536, 2 H I
  * elements less than 2^32 - 2^16 bytes, strides at most 2,796,202; operands are
- * 16-byte aligned.  `workspace` (16-byte aligned, NULL where 0) has
- * ebh_op_gated_ffn_workspace(M, H, I, dtype) bytes. */
+ * 16-byte aligned.  `workspace` (16-byte aligned, NULL where 0) has at least
+ * ebh_op_gated_ffn_workspace(M, H, I, dtype) bytes, of which fewer tokens may
+ * need more. */
 #define EBH_ACT_SILU 0
 #define EBH_ACT_GELU_TANH 1
 #define EBH_ACT_GELU_ERF 2
